@@ -1,0 +1,272 @@
+// Log-probabilities of tokens, their places in the order of the row, and a row's first tokens with
+// theirs. For a row l of V logits, m its largest,
+//
+//   log p(t) = (l_t - m) - log sum_i exp(l_i - m)
+//   before(t) = tokens with a larger logit, or an equal one and a lower id
+//
+// and the best `top` tokens are those of before = 0 .. top - 1. A row in which nothing has mass (all
+// -inf) has log p = -inf everywhere; tokens at +inf share the mass between them; a NaN in a row makes
+// every log p of it NaN and stands behind all other tokens in the order.
+//
+// Two launches. The first reads the logits once, which bounds the whole: a block takes 4,096 logits of
+// a row and leaves their maximum, the sum of exponentials against it, how many come before the token
+// asked for, and each thread's largest key (of 16 logits). The second, a block a row, joins the parts
+// in a fixed order and finds the best tokens from those keys: the top-th largest of 64 groups' maxima
+// is a bound that at least `top` logits reach, and only the logits of threads whose key reaches it (about
+// as many as `top`) are looked at again. A row in which very many logits are equal to the bound goes through its logits
+// once per token instead.
+#include "sampling.h"
+#include <type_traits>
+
+namespace ninfer {
+
+constexpr int kLpThreads = 256;
+constexpr int kLpQuads = 4;   // groups of 4 logits a thread holds
+constexpr int kLpPart = kLpThreads * kLpQuads * 4;
+constexpr int kLpTop = 64;          // most tokens that are listed: the groups the bound is taken from
+constexpr int kLpJoinThreads = 1024;
+constexpr int kLpSegments = 256;    // most threads of the first launch whose logits are looked at again
+constexpr int kLpFound = 1024;      // ... and most of these logits that reach the bound
+
+struct LogprobArgs {
+  const float* logits;   // [R, ld]
+  const int* tokens;     // [R], or null
+  float* logprob;        // [R], or null (as tokens)
+  int* before;           // [R], or null
+  int* best;             // [R, top]
+  float* best_logprob;   // [R, top]
+  float2* sums;          // [R, parts]: maximum, sum
+  int* counts;           // [R, parts]
+  uint32_t* keys;        // [R, parts * kLpThreads]
+  long long ld;
+  int R, V, top, vec;
+};
+
+// The order of tokens: NaN behind everything.
+__device__ __forceinline__ uint32_t token_key(float v) { return v != v ? 0u : ordered_key(v); }
+
+__device__ __forceinline__ float exp_above(float v, float m) { return v == m ? 1.f : __expf(v - m); }
+
+__global__ __launch_bounds__(kLpThreads) void logprob_parts_kernel(const LogprobArgs a, int parts) {
+  __shared__ float red_m[kLpThreads / 64], red_s[kLpThreads / 64];
+  __shared__ int red_c[kLpThreads / 64];
+  const int r = blockIdx.x / parts, part = blockIdx.x % parts, t0 = part * kLpPart, tid = threadIdx.x;
+  const int n = min(kLpPart, a.V - t0), lane = tid & 63, w = tid >> 6;
+  const float* row = a.logits + r * a.ld;
+  float v[kLpQuads][4];
+#pragma unroll
+  for (int u = 0; u < kLpQuads; ++u) {
+    const int i = (u * kLpThreads + tid) * 4;
+    if (a.vec && i + 4 <= n) {
+      load_row<4>(row + t0 + i, v[u]);
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) v[u][c] = i + c < n ? row[t0 + i + c] : -INFINITY;
+    }
+  }
+  const int token = a.tokens ? a.tokens[r] : -1;
+  const bool asked = token >= 0 && token < a.V;
+  const uint32_t mine = asked ? token_key(row[token]) : 0;
+  float m = -INFINITY;
+  uint32_t most = 0;
+  int count = 0;
+#pragma unroll
+  for (int u = 0; u < kLpQuads; ++u) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int i = (u * kLpThreads + tid) * 4 + c;
+      const uint32_t k = i < n ? token_key(v[u][c]) : 0;
+      most = max(most, k);
+      count += i < n && (k > mine || (k == mine && t0 + i < token));
+      m = fmaxf(m, v[u][c]);
+    }
+  }
+  if (a.top) a.keys[((int64_t)r * parts + part) * kLpThreads + tid] = most;
+  m = wave_max(m);
+  if (lane == 0) red_m[w] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(red_m[0], red_m[1]), fmaxf(red_m[2], red_m[3]));
+  float s = 0.f;
+#pragma unroll
+  for (int u = 0; u < kLpQuads; ++u) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) s += exp_above(v[u][c], m);
+  }
+  s = wave_sum(s);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) count += __shfl_xor(count, off, 64);
+  if (lane == 0) red_s[w] = s, red_c[w] = count;
+  __syncthreads();
+  if (tid == 0) {
+    const int64_t at = (int64_t)r * parts + part;
+    a.sums[at] = make_float2(m, (red_s[0] + red_s[1]) + (red_s[2] + red_s[3]));
+    a.counts[at] = (red_c[0] + red_c[1]) + (red_c[2] + red_c[3]);
+  }
+}
+
+struct LpLds {
+  uint32_t group[kLpJoinThreads / 64][64];
+  uint32_t segment[kLpSegments];
+  unsigned long long found[kLpFound];
+  unsigned long long best[kLpTop], red[kLpJoinThreads / 64];
+  float max, log_sum;
+  uint32_t bound;
+  int segments, n_found;
+};
+
+// The first key of `top` tokens of a row, one after the other: every turn the whole row.
+__device__ void best_by_turns(const LogprobArgs& a, const float* row, LpLds& l) {
+  unsigned long long last = ~0ull;
+  for (int j = 0; j < a.top; ++j) {
+    unsigned long long mine = 0;
+    for (int i = threadIdx.x; i < a.V; i += kLpJoinThreads) {
+      const unsigned long long k = (unsigned long long)token_key(row[i]) << 32 | ~(uint32_t)i;
+      if (k < last && k > mine) mine = k;
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) mine = max(mine, (unsigned long long)__shfl_xor(mine, off, 64));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) l.red[threadIdx.x >> 6] = mine;
+    __syncthreads();
+    mine = l.red[0];
+    for (int i = 1; i < kLpJoinThreads / 64; ++i) mine = max(mine, l.red[i]);
+    last = mine;
+    if (threadIdx.x == 0) l.best[j] = mine;
+  }
+  __syncthreads();
+}
+
+// Joins a row's parts; with TOP also its best tokens. Without, a block is one wave.
+template <bool TOP>
+__global__ __launch_bounds__(TOP ? kLpJoinThreads : 64) void logprob_join_kernel(const LogprobArgs a, int parts) {
+  __shared__ typename std::conditional<TOP, LpLds, int>::type lds;
+  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const float* row = a.logits + r * a.ld;
+  const int64_t base = (int64_t)r * parts;
+  float m = -INFINITY, s = 0.f, log_sum = 0.f;
+  auto log_p = [](float v, float m, float log_sum) {   // (a NaN among the logits is one in log_sum)
+    return log_sum != log_sum ? log_sum : m == -INFINITY ? m : (v == m ? 0.f : v - m) - log_sum;
+  };
+  if (tid < 64) {
+    int count = 0;
+    for (int p = lane; p < parts; p += 64) m = fmaxf(m, a.sums[base + p].x);
+    m = wave_max(m);
+    for (int p = lane; p < parts; p += 64) {
+      const float2 x = a.sums[base + p];
+      s += x.y * exp_above(x.x, m);
+      count += a.counts[base + p];
+    }
+    s = wave_sum(s);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) count += __shfl_xor(count, off, 64);
+    log_sum = logf(s);
+    if (lane == 0 && a.tokens) {
+      const int token = a.tokens[r];
+      const bool asked = token >= 0 && token < a.V;
+      a.logprob[r] = asked ? log_p(row[token], m, log_sum) : __builtin_nanf("");
+      a.before[r] = asked ? count : -1;
+    }
+  }
+  if constexpr (TOP) {
+    LpLds& l = lds;
+    if (tid == 0) l.max = m, l.log_sum = log_sum, l.segments = 0, l.n_found = 0;
+    const uint32_t* keys = a.keys + base * kLpThreads;
+    const int n = parts * kLpThreads;
+    uint32_t most = 0;
+    for (int i = tid; i < n; i += kLpJoinThreads) most = max(most, keys[i]);
+    l.group[tid >> 6][lane] = most;
+    __syncthreads();
+    if (tid < 64) {
+      for (int i = 0; i < kLpJoinThreads / 64; ++i) most = max(most, l.group[i][lane]);
+      int place = 0;
+#pragma unroll
+      for (int i = 0; i < 64; ++i) {
+        const uint32_t k = __builtin_amdgcn_readlane(most, i);
+        place += k > most || (k == most && i < lane);
+      }
+      if (place == a.top - 1) l.bound = most;
+    }
+    __syncthreads();
+    const uint32_t bound = l.bound;
+    for (int i = tid; i < n; i += kLpJoinThreads) {
+      if (keys[i] >= bound) {
+        const int at = atomicAdd(&l.segments, 1);
+        if (at < kLpSegments) l.segment[at] = i;
+      }
+    }
+    __syncthreads();
+    const int segments = l.segments;
+    if (segments <= kLpSegments) {
+      constexpr int kEach = kLpQuads * 4;
+      for (int j = tid; j < segments * kEach; j += kLpJoinThreads) {
+        const int seg = l.segment[j / kEach], x = j % kEach;
+        const int i = seg / kLpThreads * kLpPart + (x / 4 * kLpThreads + seg % kLpThreads) * 4 + x % 4;
+        if (i >= a.V) continue;
+        const uint32_t k = token_key(row[i]);
+        if (k >= bound) {
+          const int at = atomicAdd(&l.n_found, 1);
+          if (at < kLpFound) l.found[at] = (unsigned long long)k << 32 | ~(uint32_t)i;
+        }
+      }
+    }
+    __syncthreads();
+    const int found = l.n_found;
+    // (the bound may be a group without tokens, whose key no token of the row reaches from below: then all are found)
+    if (segments > kLpSegments || found > kLpFound) {
+      best_by_turns(a, row, l);
+    } else {
+      for (int j = tid; j < found; j += kLpJoinThreads) {
+        const unsigned long long k = l.found[j];
+        int place = 0;
+        for (int i = 0; i < found; ++i) place += l.found[i] > k;
+        if (place < a.top) l.best[place] = k;
+      }
+      __syncthreads();
+    }
+    if (tid < a.top) {
+      const int i = (int)~(uint32_t)l.best[tid];
+      a.best[(int64_t)r * a.top + tid] = i;
+      a.best_logprob[(int64_t)r * a.top + tid] = log_p(row[i], l.max, l.log_sum);
+    }
+  }
+}
+
+}  // namespace ninfer
+
+using namespace ninfer;
+
+extern "C" int ninfer_logprob_args_bytes() { return (int)sizeof(LogprobArgs); }
+extern "C" int ninfer_logprob_most() { return kLpTop; }
+
+// Bytes of scratch, aligned to 16: the parts' sums, counts and, with top > 0, keys.
+extern "C" long long ninfer_logprob_scratch_bytes(int R, int V, int top) {
+  const long long parts = ((long long)V + kLpPart - 1) / kLpPart * R;
+  return parts * 8 + (parts * 4 + 15) / 16 * 16 + (top > 0 ? parts * kLpThreads * 4 : 0);
+}
+
+extern "C" int ninfer_token_logprobs(const LogprobArgs* args, void* scratch, hipStream_t stream) {
+  NINFER_REQUIRE(args && scratch && (uintptr_t)scratch % 16 == 0, "token_logprobs: no arguments, or scratch not aligned");
+  LogprobArgs a = *args;
+  NINFER_REQUIRE(a.R > 0 && a.V > 0 && a.logits, "token_logprobs: R=%d V=%d must be positive, rows not null", a.R, a.V);
+  NINFER_REQUIRE(a.ld >= a.V, "token_logprobs: row stride %lld < vocabulary %d", a.ld, a.V);
+  NINFER_REQUIRE(a.top >= 0 && a.top <= kLpTop && a.top <= a.V, "token_logprobs: top %d is outside [0, min(%d, %d)]", a.top, kLpTop, a.V);
+  NINFER_REQUIRE(!a.tokens || (a.logprob && a.before), "token_logprobs: tokens without a place for their numbers");
+  NINFER_REQUIRE(a.top == 0 || (a.best && a.best_logprob), "token_logprobs: no place for the best tokens");
+  NINFER_REQUIRE(a.tokens || a.top > 0, "token_logprobs: nothing is asked for");
+  const int parts = (a.V + kLpPart - 1) / kLpPart;
+  const long long blocks = (long long)parts * a.R;
+  NINFER_REQUIRE(blocks <= 0x7fffffff, "token_logprobs: %d rows are too many", a.R);
+  a.vec = row_aligned(a.logits) && a.ld % 4 == 0;
+  char* at = (char*)scratch;
+  a.sums = (float2*)at;
+  a.counts = (int*)(at + blocks * 8);
+  a.keys = (uint32_t*)(at + blocks * 8 + (blocks * 4 + 15) / 16 * 16);
+  logprob_parts_kernel<<<(unsigned)blocks, kLpThreads, 0, stream>>>(a, parts);
+  NINFER_LAUNCH_CHECK();
+  if (a.top > 0)
+    logprob_join_kernel<true><<<a.R, kLpJoinThreads, 0, stream>>>(a, parts);
+  else
+    logprob_join_kernel<false><<<a.R, 64, 0, stream>>>(a, parts);
+  NINFER_LAUNCH_CHECK();
+  return 0;
+}

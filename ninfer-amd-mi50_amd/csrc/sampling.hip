@@ -15,7 +15,7 @@
 // number `u` in [0,1) that the caller derives from (seed, request, draw
 // index), so it does not depend on what else is in the batch. top_k <= 0
 // keeps all tokens (the reference clamps to >= 1).
-#include "common.h"
+#include "sampling.h"
 #include <type_traits>
 
 namespace ninfer {
@@ -25,12 +25,6 @@ constexpr int kBatch = 8;   // logits that a thread loads before it uses the fir
 // Tokens of a row whose draw is one step, as the first of two costs more than it saves: 64 rows of 9,000 tokens
 // 19.3 us in two, 17.6 in one; 14,000 tokens 21.7 in two (23.4 where one step took every row).
 constexpr int kShortRow = 12288;
-
-__device__ __forceinline__ uint32_t ordered_key(float v) {
-  uint32_t b = __float_as_uint(v);
-  if (b == 0x80000000u) b = 0;   // -0 and +0 are one value, as in a comparison of floats
-  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);  // ascending with the float order
-}
 
 // Probability of a token as 32.32 fixed point, from its scaled logit as the key has it, rounded (tokens of equal
 // key have equal mass, the same in every pass and kernel); m: the largest of the row.

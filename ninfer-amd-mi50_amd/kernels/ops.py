@@ -264,6 +264,35 @@ class _GatedSumArgs(ctypes.Structure):
                 ("real", ctypes.c_int), ("dtype", ctypes.c_int), ("mult", ctypes.c_float)]
 
 
+class _AdapterArgs(ctypes.Structure):
+    _fields_ = [("x", ctypes.c_void_p), ("a", ctypes.c_void_p), ("b", ctypes.c_void_p),
+                ("scale", ctypes.c_void_p), ("ranks", ctypes.c_void_p), ("row_adapter", ctypes.c_void_p),
+                ("base", ctypes.c_void_p), ("out", ctypes.c_void_p), ("h", ctypes.c_void_p),
+                ("ldx", ctypes.c_int64), ("ldb", ctypes.c_int64), ("ldo", ctypes.c_int64),
+                ("T", ctypes.c_int), ("K", ctypes.c_int), ("R", ctypes.c_int), ("S", ctypes.c_int),
+                ("L", ctypes.c_int), ("N", ctypes.c_int), ("first", ctypes.c_int * 5), ("dtype", ctypes.c_int)]
+
+
+class _AdjustArgs(ctypes.Structure):
+    _fields_ = [("logits", ctypes.c_void_p), ("out", ctypes.c_void_p), ("repetition", ctypes.c_void_p),
+                ("presence", ctypes.c_void_p), ("frequency", ctypes.c_void_p),
+                ("hist_offsets", ctypes.c_void_p), ("hist_tokens", ctypes.c_void_p),
+                ("hist_counts", ctypes.c_void_p), ("hist_generated", ctypes.c_void_p),
+                ("bias_offsets", ctypes.c_void_p), ("bias_tokens", ctypes.c_void_p),
+                ("bias_values", ctypes.c_void_p), ("masks", ctypes.c_void_p), ("mask_rows", ctypes.c_void_p),
+                ("ld", ctypes.c_int64), ("ldo", ctypes.c_int64), ("R", ctypes.c_int), ("V", ctypes.c_int),
+                ("n_hist", ctypes.c_int), ("n_bias", ctypes.c_int), ("n_masks", ctypes.c_int),
+                ("vec", ctypes.c_int)]
+
+
+class _LogprobArgs(ctypes.Structure):
+    _fields_ = [("logits", ctypes.c_void_p), ("tokens", ctypes.c_void_p), ("logprob", ctypes.c_void_p),
+                ("before", ctypes.c_void_p), ("best", ctypes.c_void_p), ("best_logprob", ctypes.c_void_p),
+                ("sums", ctypes.c_void_p), ("counts", ctypes.c_void_p), ("keys", ctypes.c_void_p),
+                ("ld", ctypes.c_int64), ("R", ctypes.c_int), ("V", ctypes.c_int), ("top", ctypes.c_int),
+                ("vec", ctypes.c_int)]
+
+
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
@@ -283,6 +312,14 @@ def _dev(t: torch.Tensor, name: str, dtype=None, dims: Optional[int] = None) -> 
         _need(t.dtype == dtype, f"{name} must be {dtype}, is {t.dtype}")
     if dims is not None:
         _need(t.dim() == dims, f"{name} must have {dims} dimensions, has {t.dim()}")
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Do two row-major [rows, columns] tensors' spans of memory meet?"""
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
 
 
 class _Together:
@@ -369,6 +406,11 @@ class HipOps:
         if self.lib.ninfer_sample_few_tokens() != self.FEW_TOKENS:
             raise KernelError(f"{self.lib_path} samples rows of up to {self.lib.ninfer_sample_few_tokens()} tokens by "
                               f"the whole GPU, these bindings say {self.FEW_TOKENS}")
+        for args, size in ((_AdapterArgs, self.lib.ninfer_adapter_args_bytes), (_AdjustArgs, self.lib.ninfer_adjust_args_bytes),
+                           (_LogprobArgs, self.lib.ninfer_logprob_args_bytes)):
+            if size() != ctypes.sizeof(args):
+                raise KernelError(f"{self.lib_path} and these bindings lay {args.__name__} out differently")
+        self.lib.ninfer_logprob_scratch_bytes.restype = ctypes.c_longlong
         self.lib.ninfer_attention_workspace_floats.restype = ctypes.c_longlong
         self.lib.ninfer_event_create.restype = ctypes.c_void_p
         self.lib.ninfer_stream_after.argtypes = [ctypes.c_void_p] * 3
@@ -2204,6 +2246,133 @@ class HipOps:
             ws = self._workspace(need, qkv.device)
             a.workspace, a.workspace_floats = ws.data_ptr(), ws.numel()
         self._ok(self.lib.ninfer_sigmoid_attention(ctypes.byref(a), self._stream()))
+
+    # ---- what single requests ask of a batch --------------------------------------------
+    def adapter_add(self, x, a, b, scale, ranks, widths, row_adapter, out, base=None):
+        """Low-rank adapters of many requests beside a projection whose output `base` [T, N] is (None: `out`, in place): for
+        row t with adapter g = row_adapter[t] and every slice s of the columns (`widths`: their sizes, up to four),
+        out[t, slice] = base[t, slice] + scale[g] B[g, slice] (A[g, s R : s R + ranks[g]] x[t]). x [T, K] and out [T, N]
+        in bfloat16 or 32-bit, columns of wider rows if need be; a [L, len(widths) R, K] and b [L, N, R] of the same
+        type, scale [L] 32-bit, ranks [L] and row_adapter [T] int32. What lies beyond an adapter's rank does not
+        count, whatever it holds. Rows whose number is outside [0, L) have no adapter: out = base."""
+        if not (x.is_cuda and x.dim() == 2 and x.dtype in _DT):
+            raise KernelError("adapter_add: x must be rows of bfloat16 or 32-bit numbers on the GPU")
+        (t, k), dt, dev = x.shape, x.dtype, x.device
+        _need(a.dim() == 3 and b.dim() == 3 and 1 <= len(widths) <= 4, "adapter_add: factors of one to four slices")
+        count, n, r = b.shape
+        _need(a.shape == (count, len(widths) * r, k) and sum(widths) == n and min(widths) >= 1 and count >= 1 and r >= 1 and k >= 1,
+              f"adapter_add: factors {tuple(a.shape)} and {tuple(b.shape)} do not fit {k} columns and slices {tuple(widths)}")
+        for name, v, dtype, size in (("a", a, dt, None), ("b", b, dt, None), ("scale", scale, torch.float32, count),
+                                     ("ranks", ranks, torch.int32, count), ("row_adapter", row_adapter, torch.int32, t)):
+            _dev(v, name, dtype)
+            if not (v.device == dev and (size is None or v.shape == (size,))):
+                raise KernelError(f"adapter_add: {name} has the wrong size or device")
+        base = out if base is None else base
+        for name, v in (("out", out), ("base", base)):
+            if not (v.device == dev and v.dtype == dt and v.shape == (t, n)):
+                raise KernelError(f"adapter_add: {name} must be [{t}, {n}] of {dt}")
+        ldx, ldo, ldb = (self._columns(v, v.shape[1], "adapter_add: rows") for v in (x, out, base))
+        if t == 0:
+            return
+        _need(min(ldo, ldb) >= n and ldx >= 0, "adapter_add: rows that overlap")
+        _need(base is out or (base.data_ptr() == out.data_ptr() and ldb == ldo) or not _overlap(base, out),
+              "adapter_add: base and out overlap")
+        _need(not _overlap(x, out), "adapter_add: x and out overlap")
+        self._here(dev)
+        h = torch.empty(t * a.shape[1], dtype=torch.float32, device=dev)
+        first = [0]
+        for w in widths:
+            first.append(first[-1] + w)
+        args = _AdapterArgs(x.data_ptr(), a.data_ptr(), b.data_ptr(), scale.data_ptr(), ranks.data_ptr(),
+                            row_adapter.data_ptr(), base.data_ptr(), out.data_ptr(), h.data_ptr(), ldx, ldb, ldo, t, k, r,
+                            len(widths), count, n, (ctypes.c_int * 5)(*first), _DT[dt])
+        self._ok(self.lib.ninfer_adapter_add(ctypes.byref(args), self._stream()))
+
+    def _here(self, device) -> None:
+        """Calls go to the current stream of the current device: their tensors have to be there."""
+        if device.index != torch.cuda.current_device():
+            raise KernelError(f"tensors on {device}, but the current device is cuda:{torch.cuda.current_device()}")
+
+    def adjust_logits(self, logits, out=None, *, repetition=None, presence=None, frequency=None, hist_offsets=None,
+                      hist_tokens=None, hist_counts=None, hist_generated=None, bias_offsets=None, bias_tokens=None,
+                      bias_values=None, masks=None, mask_rows=None):
+        """What requests ask of their rows of logits [R, V] (32-bit) before a token is drawn, into `out` (None: in place). A
+        token that stands c times in its row's history, g of them generated, of logit l: l / p^c (l p^c for l <= 0) with
+        the row's `repetition` p, less `frequency` g and, for g > 0, less `presence`, plus its bias; -inf where the
+        row's mask bars it. Per row [R]: the three penalties (32-bit, None: none) and `mask_rows` (int32, the row of
+        `masks` that holds, none where it is outside them). Histories: hist_tokens, hist_counts and hist_generated
+        (None: no token was generated), row r's from hist_offsets[r] to hist_offsets[r + 1]; counts of a token that stands
+        there more than once are added. Biases: bias_tokens and bias_values (32-bit) in the same way; of a token that stands
+        there more than once the last holds. masks [M, ceil(V / 32)] int32: bit t % 32 of word t // 32 set: token t is
+        allowed. Ids outside [0, V) are passed over."""
+        if not (logits.is_cuda and logits.dim() == 2 and logits.dtype == torch.float32):
+            raise KernelError("adjust_logits: logits must be rows of 32-bit floats on the GPU")
+        (r, v), dev = logits.shape, logits.device
+        out = logits if out is None else out
+        _need(out.device == dev and out.dtype == torch.float32 and out.shape == (r, v), "adjust_logits: out does not fit")
+        ld, ldo = (self._columns(x, v, "adjust_logits: rows") for x in (logits, out))
+        f32, i32 = torch.float32, torch.int32
+        n_hist, n_bias = (0 if x is None else x.shape[0] for x in (hist_tokens, bias_tokens))
+        for name, x, dtype, size in (
+                ("repetition", repetition, f32, r), ("presence", presence, f32, r), ("frequency", frequency, f32, r),
+                ("hist_offsets", hist_offsets, i32, r + 1), ("hist_tokens", hist_tokens, i32, n_hist),
+                ("hist_counts", hist_counts, i32, n_hist), ("hist_generated", hist_generated, i32, n_hist),
+                ("bias_offsets", bias_offsets, i32, r + 1), ("bias_tokens", bias_tokens, i32, n_bias),
+                ("bias_values", bias_values, f32, n_bias), ("mask_rows", mask_rows, i32, r)):
+            if x is not None:
+                _dev(x, name, dtype, 1)
+                if not (x.shape[0] == size and x.device == dev):
+                    raise KernelError(f"adjust_logits: {name} has the wrong size or device")
+        _need((hist_offsets is None) == (hist_tokens is None) == (hist_counts is None)
+              and (hist_generated is None or hist_tokens is not None), "adjust_logits: a history is offsets, tokens and counts")
+        _need((bias_offsets is None) == (bias_tokens is None) == (bias_values is None),
+              "adjust_logits: biases are offsets, tokens and values")
+        _need((masks is None) == (mask_rows is None), "adjust_logits: masks and the rows' choice of them go together")
+        if masks is not None:
+            _dev(masks, "masks", i32, 2)
+            _need(masks.shape[1] == (v + 31) // 32 and masks.device == dev, "adjust_logits: masks have a bit for every token")
+        if r == 0 or v == 0:
+            return
+        _need(min(ld, ldo) >= v, "adjust_logits: rows that overlap")
+        _need(out is logits or (out.data_ptr() == logits.data_ptr() and ld == ldo) or not _overlap(logits, out),
+              "adjust_logits: logits and out overlap")
+        self._here(dev)
+        args = _AdjustArgs(logits.data_ptr(), out.data_ptr(), _ptr(repetition), _ptr(presence), _ptr(frequency),
+                           _ptr(hist_offsets), _ptr(hist_tokens), _ptr(hist_counts), _ptr(hist_generated),
+                           _ptr(bias_offsets), _ptr(bias_tokens), _ptr(bias_values), _ptr(masks), _ptr(mask_rows), ld, ldo,
+                           r, v, n_hist, n_bias, 0 if masks is None else masks.shape[0], 0)
+        self._ok(self.lib.ninfer_adjust_logits(ctypes.byref(args), self._stream()))
+
+    LISTED_TOKENS = 64   # most tokens of a row whose log-probabilities `token_logprobs` lists
+
+    def token_logprobs(self, logits, tokens=None, top=0):
+        """Log-probabilities of tokens under the softmax of their rows of logits [R, V] (32-bit): (that of tokens[r] [R], how
+        many tokens stand before it [R], the `top` first tokens of the row [R, top], theirs [R, top]); the order of tokens is
+        by logit, of equal ones the lower id first. Without `tokens` (int32) the first two are None; for a token outside
+        [0, V) they are NaN and -1. A row of nothing but -inf has log-probabilities of -inf; a NaN makes all of its row's NaN
+        and stands behind every other token."""
+        if not (logits.is_cuda and logits.dim() == 2 and logits.dtype == torch.float32):
+            raise KernelError("token_logprobs: logits must be rows of 32-bit floats on the GPU")
+        (r, v), dev = logits.shape, logits.device
+        ld = self._columns(logits, v, "token_logprobs: rows")
+        if not (0 <= top <= min(self.LISTED_TOKENS, v)):
+            raise KernelError(f"token_logprobs: top {top} is outside [0, {min(self.LISTED_TOKENS, v)}]")
+        logprob = before = None
+        if tokens is not None:
+            _dev(tokens, "tokens", torch.int32, 1)
+            _need(tokens.shape[0] == r and tokens.device == dev, "token_logprobs: one token a row")
+            logprob = torch.empty(r, dtype=torch.float32, device=dev)
+            before = torch.empty(r, dtype=torch.int32, device=dev)
+        best = torch.empty((r, top), dtype=torch.int32, device=dev)
+        best_logprob = torch.empty((r, top), dtype=torch.float32, device=dev)
+        if r and v and (top or tokens is not None):
+            _need(ld >= v, "token_logprobs: rows that overlap")
+            self._here(dev)
+            scratch = torch.empty(self.lib.ninfer_logprob_scratch_bytes(r, v, top), dtype=torch.uint8, device=dev)
+            args = _LogprobArgs(logits.data_ptr(), _ptr(tokens), _ptr(logprob), _ptr(before), best.data_ptr(),
+                                best_logprob.data_ptr(), None, None, None, ld, r, v, top, 0)
+            self._ok(self.lib.ninfer_token_logprobs(ctypes.byref(args), ctypes.c_void_p(scratch.data_ptr()), self._stream()))
+        return logprob, before, best, best_logprob
 
     # ---- sampling -------------------------------------------------------------------
     def uniforms(self, seeds, keys, draws, out):
