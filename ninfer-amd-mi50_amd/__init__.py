@@ -7,12 +7,13 @@ from .config import ConfigError, EngineOptions, Qwen2MoeConfig
 from .api import Ninfer, Session
 from .engine import Chunk, ModelRunner
 from .engine.scheduler import Request, Scheduler
-from .sampling import Sampler, SamplingParams
+from .sampling import Sampler, SamplingParams, TokenLogprob
 from .loading import build_spec, load_model, random_model, write_random_model
 from .registry import (architectures, make_part, register_architecture, register_part,
                        resolve_architecture)
 from .weights import WeightError
+from .weights.adapter_files import AdapterWeights, read_adapter
 
-__all__ = ["Ninfer", "Session", "Request", "Scheduler", "Sampler", "SamplingParams", "ConfigError", "EngineOptions", "Qwen2MoeConfig", "Chunk", "ModelRunner", "build_spec",
+__all__ = ["Ninfer", "Session", "Request", "Scheduler", "Sampler", "SamplingParams", "TokenLogprob", "AdapterWeights", "read_adapter", "ConfigError", "EngineOptions", "Qwen2MoeConfig", "Chunk", "ModelRunner", "build_spec",
            "load_model", "random_model", "write_random_model", "architectures", "make_part",
            "register_architecture", "register_part", "resolve_architecture", "WeightError"]

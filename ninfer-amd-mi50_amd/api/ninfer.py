@@ -4,13 +4,14 @@
 `sample` on the engine; the same names and meanings of options where the
 reference has them (`max_context`, `prefill_chunk`, `num_sequences`). Logits
 come back as numpy arrays. Added for what the reference leaves to an outside
-scheduler: `step` (a mixed batch) and `generate` (the scheduler).
+scheduler: `step` (a mixed batch), `generate` and `complete` (the scheduler), `score` (log-probabilities
+of given tokens), and low-rank adapters that sessions and requests name (`load_adapter`).
 Return-code conventions of the C API (src/api/ninfer_c_api.cpp:191,226,235)
 become exceptions here.
 """
 from __future__ import annotations
 
-from typing import Dict, List, Optional, Sequence
+from typing import Callable, Dict, List, Optional, Sequence, Union
 
 import numpy as np
 
@@ -19,15 +20,22 @@ from ..engine.runner import Chunk
 from ..engine.scheduler import Request, Scheduler
 from ..loading import load_model, random_model
 from ..sampling.params import SamplingParams
-from ..sampling.sampler import History, SampleRow, Sampler, fresh_seed
+from ..sampling.sampler import History, SampleRow, Sampler, TokenLogprob, allowed_words, fresh_seed
 
 
 class Session:
     """One request's place in the cache (reference tools/ninfer_ctypes.py:48-90)."""
 
-    def __init__(self, engine: "Ninfer"):
+    def __init__(self, engine: "Ninfer", adapter: Optional[str] = None):
+        engine.runner.hold_adapter(adapter)
         self._engine = engine
-        self._slot: Optional[int] = engine.runner.open()
+        self.adapter = adapter   # the name of the low-rank adapter that all its tokens run with
+        self._slot: Optional[int] = None
+        try:
+            self._slot = engine.runner.open()
+        except BaseException:
+            engine.runner.let_go_adapter(adapter)
+            raise
 
     def __enter__(self):
         return self
@@ -58,16 +66,17 @@ class Session:
             part = list(tokens[i:i + chunk])
             last = i + chunk >= len(tokens)
             logits = self._engine.runner.step(
-                [Chunk(self._slot, part, [len(part) - 1] if last else [])])
+                [Chunk(self._slot, part, [len(part) - 1] if last else [], self.adapter)])
         return logits[0].float().cpu().numpy()
 
     def decode(self, token: int) -> np.ndarray:
-        logits = self._engine.runner.step([Chunk(self._slot, [int(token)], [0])])
+        logits = self._engine.runner.step([Chunk(self._slot, [int(token)], [0], self.adapter)])
         return logits[0].float().cpu().numpy()
 
     def close(self) -> None:
         if self._slot is not None:
             self._engine.runner.close(self._slot)
+            self._engine.runner.let_go_adapter(self.adapter)
             self._slot = None
 
 
@@ -77,7 +86,7 @@ class Ninfer:
                  page_size: int = 16, num_pages: Optional[int] = None, use_graph: bool = False,
                  random_config: Optional[dict] = None, random_seed: int = 0,
                  random_weights_dtype: Optional[str] = None, kv_bytes: Optional[int] = None,
-                 check_pages: bool = False):
+                 check_pages: bool = False, max_adapters: int = 0, max_adapter_rank: int = 64):
         if max_context is None:
             # as many positions as the model's parts allow (a table of learned positions has
             # so many rows), and no more than the reference's default
@@ -90,7 +99,8 @@ class Ninfer:
                                      prefill_chunk=prefill_chunk, num_sequences=num_sequences,
                                      page_size=page_size, num_pages=num_pages,
                                      use_graph=use_graph, kv_bytes=kv_bytes,
-                                     check_pages=check_pages)
+                                     check_pages=check_pages, max_adapters=max_adapters,
+                                     max_adapter_rank=max_adapter_rank)
         if model_dir is not None:
             self.runner = load_model(model_dir, self.options)
         elif random_config is not None:
@@ -153,37 +163,58 @@ class Ninfer:
             raise ValueError(f"{name}: [{offset}, {end}) is outside its {flat.numel()} numbers")
         return flat[offset:end].float().cpu().numpy()
 
+    # ---- adapters -------------------------------------------------------------------
+    def load_adapter(self, name: str, folder: str) -> None:
+        """Read a low-rank adapter (adapter_config.json and adapter_model.safetensors) and hold it under `name`, for sessions
+        and requests that ask for it. The engine has room for `max_adapters` of rank `max_adapter_rank`."""
+        self.runner.load_adapter(name, folder)
+
+    def remove_adapter(self, name: str) -> None:
+        """Make its place free. Refused while a session or request that has it is open."""
+        self.runner.remove_adapter(name)
+
+    def adapters(self) -> List[str]:
+        return [] if self.runner.adapters is None else self.runner.adapters.names()
+
     # ---- sessions -------------------------------------------------------------------
-    def session(self) -> Session:
-        return Session(self)
+    def session(self, adapter: Optional[str] = None) -> Session:
+        return Session(self, adapter)
 
     def decode_batch(self, sessions: Sequence[Session], tokens: Sequence[int]) -> np.ndarray:
         """One token for each of several sessions in one step; logits [n, vocab]
         (reference src/api/ninfer_c_api.cpp:219-246)."""
         if len(sessions) != len(tokens):
             raise ValueError("one token per session")
-        logits = self.runner.step([Chunk(s.slot, [int(t)], [0])
+        logits = self.runner.step([Chunk(s.slot, [int(t)], [0], s.adapter)
                                    for s, t in zip(sessions, tokens)])
         return logits.float().cpu().numpy()
 
     def step(self, entries: Sequence[tuple]) -> Optional[np.ndarray]:
         """A mixed batch: entries of (session, tokens, wanted rows); logits of the
         wanted rows in order, or None."""
-        logits = self.runner.step([Chunk(s.slot, list(t), list(w)) for s, t, w in entries])
+        logits = self.runner.step([Chunk(s.slot, list(t), list(w), s.adapter) for s, t, w in entries])
         return None if logits is None else logits.float().cpu().numpy()
 
     def sample(self, logits, temperature: float = 0.7, top_k: int = 50, top_p: float = 0.95,
                repetition_penalty: float = 1.0, seed: int = 0,
-               recent: Sequence[int] = ()) -> int:
+               recent: Sequence[int] = (), presence_penalty: float = 0.0, frequency_penalty: float = 0.0,
+               logit_bias: Optional[Dict[int, float]] = None, allowed=None, generated: Sequence[int] = ()) -> int:
         """Stateless sampling of one row (reference src/api/ninfer_c_api.cpp:248-260;
-        there the history is empty, here `recent` may carry it)."""
+        there the history is empty, here `recent` may carry it, and `generated` the tokens behind it that were
+        generated, to which alone the presence and frequency penalties apply). `allowed`: what may come, token ids or
+        the words of a mask (None: every token)."""
         import torch
         row = torch.as_tensor(np.asarray(logits, dtype=np.float32)).reshape(1, -1).to(
             self.runner.device)
-        params = SamplingParams(temperature, top_k, top_p, repetition_penalty, seed, 1)
+        params = SamplingParams(temperature, top_k, top_p, repetition_penalty, seed, 1, presence_penalty,
+                                frequency_penalty, logit_bias)
+        params.check(row.shape[1], 0)
+        history = History(recent)
+        for t in generated:
+            history.add(int(t))
         self._sample_calls += 1
-        r = SampleRow(params, History(recent), 0, 0 if seed else self._sample_calls,
-                      seed or fresh_seed())
+        r = SampleRow(params, history, 0, 0 if seed else self._sample_calls,
+                      seed or fresh_seed(), allowed_words(allowed, row.shape[1]))
         return self.sampler.sample(row, [r])[0]
 
     def close(self) -> None:
@@ -202,18 +233,58 @@ class Ninfer:
             torch.cuda.empty_cache()
 
     # ---- generation -----------------------------------------------------------------
-    def generate(self, prompts: Sequence[Sequence[int]], params: Optional[SamplingParams] = None,
-                 stop_ids: Optional[Sequence[int]] = None) -> List[List[int]]:
+    def generate(self, prompts: Sequence[Sequence[int]],
+                 params: Union[SamplingParams, Sequence[SamplingParams], None] = None,
+                 stop_ids: Optional[Sequence[int]] = None, adapters: Optional[Sequence[Optional[str]]] = None,
+                 allow: Optional[Sequence[Optional[Callable]]] = None) -> List[List[int]]:
         """Generated token ids for each prompt, through the scheduler."""
-        params = params or SamplingParams()
+        return [r.output for r in self.complete(prompts, params, stop_ids, adapters, allow)]
+
+    def complete(self, prompts: Sequence[Sequence[int]],
+                 params: Union[SamplingParams, Sequence[SamplingParams], None] = None,
+                 stop_ids: Optional[Sequence[int]] = None, adapters: Optional[Sequence[Optional[str]]] = None,
+                 allow: Optional[Sequence[Optional[Callable]]] = None) -> List[Request]:
+        """The finished requests of the prompts (`output`, `logprobs`), through the scheduler. `params`: one for all of
+        them or one for each; `adapters`: the name of each one's adapter or None; `allow`: each one's `Request.allow`."""
+        n = len(prompts)
+        if params is None or isinstance(params, SamplingParams):
+            params = [params or SamplingParams()] * n
+        adapters = [None] * n if adapters is None else list(adapters)
+        allow = [None] * n if allow is None else list(allow)
+        if not len(params) == len(adapters) == len(allow) == n:
+            raise ValueError(f"{n} prompts, {len(params)} params, {len(adapters)} adapters, {len(allow)} allow")
         if stop_ids is None:
             stop_ids = list(self.runner.spec.eos_token_ids)
         sched = Scheduler(self.runner, self.sampler)
-        reqs = [Request(str(i), list(p), params, stop_ids) for i, p in enumerate(prompts)]
+        reqs = [Request(str(i), list(p), q, stop_ids, a, f) for i, (p, q, a, f) in enumerate(zip(prompts, params, adapters, allow))]
         for r in reqs:
             sched.add(r)
         sched.run()
         for r in reqs:
             if r.status == "failed":
                 raise RuntimeError(f"request {r.id}: {r.error}")
-        return [r.output for r in reqs]
+        return reqs
+
+    def score(self, prompts: Sequence[Sequence[int]], top: int = 0,
+              adapters: Optional[Sequence[Optional[str]]] = None) -> List[List[TokenLogprob]]:
+        """How likely the model takes each prompt's tokens to be: for every token but the first its log-probability behind the
+        tokens before it, its place in the order, and the `top` best tokens in its place. Prompts run one after the
+        other, in portions of `prefill_chunk`."""
+        adapters = [None] * len(prompts) if adapters is None else list(adapters)
+        if len(adapters) != len(prompts):
+            raise ValueError(f"{len(prompts)} prompts, {len(adapters)} adapters")
+        most = min(getattr(self.runner.ops, "LISTED_TOKENS", 0), self.vocab)
+        if not 0 <= top <= most:
+            raise ValueError(f"top must be in [0, {most}], is {top}")
+        out: List[List[TokenLogprob]] = []
+        for prompt, adapter in zip(prompts, adapters):
+            if len(prompt) == 0:
+                raise ValueError("a prompt to score needs at least one token")
+            told: List[TokenLogprob] = []
+            with self.session(adapter) as s:
+                for i in range(0, len(prompt) - 1, self.options.prefill_chunk):
+                    part = list(prompt[i:min(i + self.options.prefill_chunk, len(prompt) - 1)])
+                    logits = self.runner.step([Chunk(s.slot, part, range(len(part)), adapter)])
+                    told += self.sampler.logprobs(logits, prompt[i + 1:i + 1 + len(part)], top)
+            out.append(told)
+        return out

@@ -37,6 +37,12 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--top-k", type=int, default=50)
     ap.add_argument("--top-p", type=float, default=0.95)
     ap.add_argument("--repeat-penalty", type=float, default=1.05)
+    ap.add_argument("--presence-penalty", type=float, default=0.0, help="off a token's logit once it was generated")
+    ap.add_argument("--frequency-penalty", type=float, default=0.0, help="off a token's logit for every time it was generated")
+    ap.add_argument("--logit-bias", metavar="ID:BIAS,...", help="added to the logits of tokens (-inf bars one)")
+    ap.add_argument("--logprobs", type=int, metavar="N",
+                    help="write each generated token's log-probability, and the N best in its place, to stderr")
+    ap.add_argument("--adapter", metavar="DIR", help="low-rank adapter that the prompts run with")
     ap.add_argument("--seed", type=int, default=0, help="sampling seed (0: 1234 for a one-shot run, a fresh one per turn of the loop)")
     ap.add_argument("--graph", action="store_true", help="replay decode steps from a HIP graph")
     ap.add_argument("--verify", action="store_true",
@@ -64,7 +70,6 @@ def main(argv: Optional[List[str]] = None) -> int:
 
     from .api.ninfer import Ninfer
     from .config.base import read_config_json
-    from .sampling.params import SamplingParams
 
     dtype = {"bf16": "bfloat16", "fp32": "float32"}.get(args.dtype, args.dtype)
     raw = read_config_json(args.model_dir)
@@ -82,10 +87,15 @@ def main(argv: Optional[List[str]] = None) -> int:
                   num_pages=args.kv_pages, use_graph=args.graph,
                   kv_bytes=int(args.kv_gib * (1 << 30)) if args.kv_gib is not None else None)
     try:
+        if args.adapter:
+            from .weights.adapter_files import read_adapter
+            common.update(max_adapters=1, max_adapter_rank=read_adapter(args.adapter).rank)
         if args.random_weights is not None:
             eng = Ninfer(random_config=raw, random_seed=args.random_weights, **common)
         else:
             eng = Ninfer(args.model_dir, **common)
+        if args.adapter:
+            eng.load_adapter(_ADAPTER, args.adapter)
         if args.random_prompts:   # the vocabulary is the bound model's, whatever its config calls it
             rng = random.Random(args.seed or 1234)
             for n in args.random_prompts.split(","):
@@ -95,11 +105,13 @@ def main(argv: Optional[List[str]] = None) -> int:
         stop = [args.eos_id] if args.eos_id is not None else None
         if not prompts:
             return _interactive(eng, args, stop)
-        params = SamplingParams(args.temperature, args.top_k, args.top_p, args.repeat_penalty,
-                                args.seed or 1234, args.max_new)
+        params = _params(args, args.seed or 1234)
         t1 = time.time()
-        outs = eng.generate(prompts, params, stop)
+        done = eng.complete(prompts, params, stop, _adapters(args, prompts))
         dt = time.time() - t1
+        outs = [r.output for r in done]
+        for r in done:
+            _say_logprobs(r)
         for o in outs:
             print(",".join(map(str, o)))
         n = sum(len(o) for o in outs)
@@ -115,6 +127,30 @@ def main(argv: Optional[List[str]] = None) -> int:
         print(f"ninfer: error: {e}", file=sys.stderr)
         return 1
     return 0
+
+
+_ADAPTER = "adapter"   # the name of --adapter's
+
+
+def _adapters(args, prompts) -> list:
+    return [_ADAPTER if args.adapter else None] * len(prompts)
+
+
+def _params(args, seed: int):
+    from .sampling.params import SamplingParams
+    bias = {}
+    for pair in (args.logit_bias or "").split(","):
+        if pair.strip():
+            token, _, value = pair.partition(":")
+            bias[int(token)] = float(value)
+    return SamplingParams(args.temperature, args.top_k, args.top_p, args.repeat_penalty, seed, args.max_new,
+                          args.presence_penalty, args.frequency_penalty, bias or None, args.logprobs)
+
+
+def _say_logprobs(request) -> None:
+    for i, t in enumerate(request.logprobs):
+        best = "".join(f" {b}:{p:.4f}" for b, p in t.best)
+        print(f"[ninfer] request {request.id} token {i}: {t.token} logprob {t.logprob:.4f} place {t.place}{best}", file=sys.stderr)
 
 
 def _verify(args, raw, common, prompts, params, stop, outs) -> None:
@@ -136,7 +172,9 @@ def _verify(args, raw, common, prompts, params, stop, outs) -> None:
                      random_weights_dtype=common["dtype"], **golden)
     else:
         eng = Ninfer(args.model_dir, **golden)
-    want = eng.generate(prompts, params, stop)
+    if args.adapter:
+        eng.load_adapter(_ADAPTER, args.adapter)
+    want = eng.generate(prompts, params, stop, _adapters(args, prompts))
     same = True
     for r, (a, b) in enumerate(zip(outs, want)):
         if a != b:
@@ -153,7 +191,6 @@ def _verify(args, raw, common, prompts, params, stop, outs) -> None:
 def _interactive(eng, args, stop) -> int:
     """Turn after turn from standard input: a line of comma-separated token ids is added to
     what has been said, the answer is generated from all of it and added too."""
-    from .sampling.params import SamplingParams
     print("ninfer ready: one line of comma-separated token ids per turn, end of input to exit",
           file=sys.stderr, flush=True)
     said: List[int] = []
@@ -162,9 +199,9 @@ def _interactive(eng, args, stop) -> int:
         if not ids:
             continue
         said += ids
-        params = SamplingParams(args.temperature, args.top_k, args.top_p, args.repeat_penalty,
-                                args.seed, args.max_new)
-        answer = eng.generate([said], params, stop)[0]
+        done = eng.complete([said], _params(args, args.seed), stop, _adapters(args, [said]))[0]
+        _say_logprobs(done)
+        answer = done.output
         print(",".join(map(str, answer)), flush=True)
         said += answer
     return 0

@@ -24,6 +24,8 @@ class EngineOptions:
     poison_freed_pages: bool = False  # debugging: fill pages that are given back with NaN
     check_pages: bool = False      # debugging: before every step, check on the host that every page the step reads or writes is held by its request and by no other
     device: str = "cuda:0"
+    max_adapters: int = 0          # most low-rank adapters held at once (0: requests have none)
+    max_adapter_rank: int = 64     # ... and the largest rank of one
 
     def validate(self) -> None:
         if self.dtype not in ("bfloat16", "float32"):
@@ -31,6 +33,9 @@ class EngineOptions:
         for name in ("max_context", "prefill_chunk", "num_sequences", "page_size", "max_graphs"):
             if getattr(self, name) < 1:
                 raise ValueError(f"{name} must be >= 1, got {getattr(self, name)}")
+        if self.max_adapters < 0 or self.max_adapter_rank < 1:
+            raise ValueError(f"max_adapters must be >= 0 and max_adapter_rank >= 1, got {self.max_adapters} and "
+                             f"{self.max_adapter_rank}")
         if self.num_pages is not None and self.num_pages < 1:
             raise ValueError(f"num_pages must be >= 1, got {self.num_pages}")
         if self.kv_bytes is not None and self.kv_bytes < 1:

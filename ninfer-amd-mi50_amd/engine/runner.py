@@ -23,18 +23,21 @@ from ..cache.manager import CacheManager
 from ..config.options import EngineOptions
 from ..models.spec import ModelSpec
 from ..parts.base import CacheView, CallInfo, StepContext, WeightBinder
+from ..weights.adapter_files import AdapterWeights, read_adapter
 from ..weights.source import check_tensors
+from .adapters import AdapterSet
 
 _DTYPES = {"bfloat16": torch.bfloat16, "float32": torch.float32}
 
 
 @dataclass
 class Chunk:
-    """The next tokens of one request in a step and the rows (indices into
-    `tokens`) whose logits are wanted."""
+    """The next tokens of one request in a step, the rows (indices into
+    `tokens`) whose logits are wanted, and the name of the request's adapter (the same in all its steps)."""
     slot: int
     tokens: Sequence[int]
     want: Sequence[int] = field(default_factory=list)
+    adapter: Optional[str] = None
 
 
 class ModelRunner:
@@ -59,6 +62,9 @@ class ModelRunner:
         binder = WeightBinder(source, self.device, self.act_dtype)
         spec.bind(binder)
         self._held = binder.held
+        self.adapters: Optional[AdapterSet] = None
+        if options.max_adapters:
+            self.adapters = AdapterSet(spec, options.max_adapters, options.max_adapter_rank, self.device, self.act_dtype)
 
         # one cache instance per plan entry that writes keys and values
         needs = []
@@ -111,6 +117,34 @@ class ModelRunner:
     def close(self, slot: int) -> None:
         self.cache.release(slot)
 
+    # ---- adapters --------------------------------------------------------------
+    def load_adapter(self, name: str, weights) -> None:
+        """Hold a low-rank adapter under `name`: a folder (see weights/adapter_files.py) or `AdapterWeights`."""
+        if self.adapters is None:
+            raise ValueError("the engine was made without room for adapters (max_adapters)")
+        self.adapters.load(name, weights if isinstance(weights, AdapterWeights) else read_adapter(weights))
+
+    def remove_adapter(self, name: str) -> None:
+        self.adapter_number(name)
+        self.adapters.remove(name)
+
+    def adapter_number(self, name: Optional[str]) -> int:
+        """The number of a loaded adapter in the tables, -1 for None; ValueError for a name that is not loaded."""
+        if name is None:
+            return -1
+        if self.adapters is None:
+            raise ValueError(f"no adapter named {name!r} is loaded: the engine was made without room for adapters")
+        return self.adapters.number(name)
+
+    def hold_adapter(self, name: Optional[str]) -> None:
+        """A request or session has this adapter from now on, until `let_go_adapter`."""
+        if self.adapter_number(name) >= 0:
+            self.adapters.hold(name)
+
+    def let_go_adapter(self, name: Optional[str]) -> None:
+        if name is not None:
+            self.adapters.let_go(name)
+
     def release(self) -> None:
         """Drop everything this runner holds on the device: captured graphs (and with them
         their memory pools), staging buffers, the cache's pools, the bound weights. The
@@ -122,6 +156,9 @@ class ModelRunner:
             self.ops.graph_holder_gone(self)
         self._staging = []
         self._held = {}
+        if self.adapters is not None:
+            self.adapters.drop()
+            self.adapters = None
         self.cache.drop_pools()
         self.spec = None
 
@@ -175,6 +212,8 @@ class ModelRunner:
                 want_rows.append(first_row[c.slot] + w)
         if tokens.min() < 0 or tokens.max() >= self.vocab_size:
             raise ValueError(f"token id outside [0, {self.vocab_size})")
+        numbers = [self.adapter_number(c.adapter) for c in chunks]
+        adapters = any(g >= 0 for g in numbers)
         # the batch is well formed: now pages for all its requests, or for none
         cache.reserve_all([(c.slot, p + len(c.tokens)) for c, p in zip(chunks, pos0)])
         max_kv_len = int(max(p + len(c.tokens) for c, p in zip(chunks, pos0)))
@@ -192,11 +231,13 @@ class ModelRunner:
         parts = [tokens, positions, row_seq, np.asarray(slots, np.int32), row_start, qlen,
                  np.asarray(pos0, np.int32), np.asarray(want_rows, np.int32)]
         parts += [t.reshape(-1) for t in tables]
+        if adapters:
+            parts.append(np.repeat(np.asarray(numbers, np.int32), qlen))
         sizes = [x.size for x in parts]
         host = torch.from_numpy(np.concatenate(parts))
         shape = dict(T=T, S=S, sizes=sizes, widths=[t.shape[1] for t in tables],
                      max_qlen=int(qlen.max()), max_kv_len=max_kv_len, wants=bool(want_rows),
-                     single_rows=single_rows,
+                     single_rows=single_rows, adapters=adapters,
                      portion_keys=sum(p + len(c.tokens) for c, p in zip(chunks[single_rows:], pos0[single_rows:])))
         if graph:
             logits = self._step_graph(host, shape)
@@ -268,7 +309,8 @@ class ModelRunner:
     def _forward(self, dev: torch.Tensor, shape: dict) -> Optional[torch.Tensor]:
         """Run the model on the step described by the packed index buffer `dev`
         (tokens, positions, row_seq, slots, row_start, qlen, pos0, wanted rows,
-        then one block table per cache group)."""
+        then one block table per cache group, then, if a row has one, the
+        rows' adapters)."""
         views = []
         o = 0
         for n in shape["sizes"]:
@@ -276,26 +318,27 @@ class ModelRunner:
             o += n
         S = shape["S"]
         d_tables = [v.view(S, w) for v, w in zip(views[8:], shape["widths"])]
+        row_adapter = views[-1] if shape["adapters"] else None
         ctx = StepContext(
             ops=self.ops, act_dtype=self.act_dtype, device=self.device, T=shape["T"], S=S,
             tokens=views[0], positions=views[1], row_seq=views[2], seq_slots=views[3],
             seq_row_start=views[4], seq_qlen=views[5], seq_pos0=views[6],
             max_qlen=shape["max_qlen"], max_kv_len=shape["max_kv_len"],
             all_decode=shape["max_qlen"] == 1, single_rows=shape["single_rows"],
-            portion_keys=shape["portion_keys"])
+            portion_keys=shape["portion_keys"], row_adapter=row_adapter)
         es = self.cache.state[:, self._embedding_state] if self._embedding_state is not None else None
         return self.spec.forward(ctx, self._call_infos(d_tables),
                                  views[7] if shape["wants"] else None, es, self.tap)
 
     def _step_graph(self, host: torch.Tensor, shape: dict) -> torch.Tensor:
         """Decode-only steps replayed from a captured HIP graph: one graph per
-        (requests in the step, context bound). The index buffer is the graph's
+        (requests in the step, context bound, whether a row has an adapter). The index buffer is the graph's
         only input; it is refreshed by one copy before every replay. The first
         step of a shape runs eagerly (it also sizes every workspace), the
         second is captured. The reference captures its single-token dense
         decode the same way (src/models/model.hip:786-830). The returned logits
         live in the graph's memory and are valid until the next step."""
-        key = (shape["S"], shape["max_kv_len"])
+        key = (shape["S"], shape["max_kv_len"]) + (("adapters",) if shape["adapters"] else ())
         entry = self._graphs.get(key)
         if entry is not None:
             self._graphs.move_to_end(key)

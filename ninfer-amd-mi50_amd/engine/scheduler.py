@@ -30,11 +30,11 @@ from __future__ import annotations
 import hashlib
 from collections import deque
 from dataclasses import dataclass, field
-from typing import Deque, Dict, List, Optional, Sequence, Tuple
+from typing import Callable, Deque, Dict, List, Optional, Sequence, Tuple
 
 from ..cache.pages import OutOfPages
 from ..sampling.params import SamplingParams
-from ..sampling.sampler import History, SampleRow, fresh_seed
+from ..sampling.sampler import History, SampleRow, TokenLogprob, allowed_words, fresh_seed
 from .runner import Chunk
 
 
@@ -44,6 +44,10 @@ class Request:
     prompt: List[int]
     params: SamplingParams = field(default_factory=SamplingParams)
     stop_ids: Sequence[int] = ()
+    adapter: Optional[str] = None   # name of the low-rank adapter it runs with
+    # what may come next, asked before every draw with the tokens generated so far: token ids, words of a mask
+    # (an array of uint32, bit t % 32 of word t // 32), or None for every token
+    allow: Optional[Callable[[Sequence[int]], object]] = None
     # progress
     output: List[int] = field(default_factory=list)
     slot: Optional[int] = None
@@ -55,6 +59,7 @@ class Request:
     key: int = 0                    # of its stream of random numbers: from its id (see add)
     order: int = 0                  # of its arrival at the scheduler
     history: History = field(default_factory=History)
+    logprobs: List[TokenLogprob] = field(default_factory=list)   # one per token of `output`, where params.logprobs asks for them
 
     @property
     def tokens(self) -> List[int]:
@@ -106,6 +111,13 @@ class Scheduler:
             # the reference's rule (src/runtime/engine.cpp:124-127)
             request.status = "failed"
             request.error = "prompt + max_new_tokens exceeds max_context"
+            self.finished.append(request)
+            return
+        try:
+            request.params.check(self.runner.vocab_size, getattr(self.runner.ops, "LISTED_TOKENS", 0))
+            self.runner.hold_adapter(request.adapter)
+        except ValueError as e:
+            request.status, request.error = "failed", str(e)
             self.finished.append(request)
             return
         request.seed = request.params.seed if request.params.seed != 0 else fresh_seed()
@@ -233,13 +245,15 @@ class Scheduler:
         """Plan, run and sample one step; returns the requests it finished."""
         planned = self.plan()
         done: List[Request] = list(planned.failed)
+        for req in planned.failed:
+            self.runner.let_go_adapter(req.adapter)
         if not planned.chunks:
             if self.has_work() and not planned.failed and not planned.preempted:
                 raise RuntimeError("scheduler made no progress")
             return done
         chunks = []
         for req, n, want in planned.chunks:
-            chunks.append(Chunk(req.slot, req.next_tokens(n), [n - 1] if want else []))
+            chunks.append(Chunk(req.slot, req.next_tokens(n), [n - 1] if want else [], req.adapter))
         logits = self.runner.step(chunks)
         self.steps += 1
         rows = []
@@ -248,16 +262,32 @@ class Scheduler:
             req.cached += n
             if want:
                 wanting.append(req)
-                rows.append(SampleRow(req.params, req.history, req.key, len(req.output), req.seed))
+                allowed = None
+                if req.allow is not None:
+                    try:
+                        allowed = allowed_words(req.allow(req.output), self.runner.vocab_size)
+                    except Exception as e:   # (the request's own: the others go on)
+                        req.error = f"what may come next: {e}"
+                rows.append(SampleRow(req.params, req.history, req.key, len(req.output), req.seed, allowed))
         if wanting:
             tokens = self.sampler.sample(logits, rows)
-            for req, tok in zip(wanting, tokens):
+            asked = [req.params.logprobs for req in wanting if req.params.logprobs is not None]
+            told = self.sampler.logprobs(logits, tokens, max(asked)) if asked else None
+            for i, (req, tok) in enumerate(zip(wanting, tokens)):
+                if req.error is not None:
+                    self._finish(req)
+                    req.status = "failed"
+                    done.append(req)
+                    continue
                 if tok in req.stop_ids:
                     self._finish(req)            # the stop token is not part of the output
                     done.append(req)
                     continue
                 req.output.append(tok)
                 req.history.add(tok)
+                if req.params.logprobs is not None:
+                    told[i].best = told[i].best[:req.params.logprobs]
+                    req.logprobs.append(told[i])
                 if len(req.output) >= req.params.max_new_tokens:
                     self._finish(req)
                     done.append(req)
@@ -265,6 +295,7 @@ class Scheduler:
 
     def _finish(self, req: Request) -> None:
         self.cache.release(req.slot)
+        self.runner.let_go_adapter(req.adapter)
         req.slot, req.status = None, "finished"
         self.running.remove(req)
         self.finished.append(req)

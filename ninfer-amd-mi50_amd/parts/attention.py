@@ -25,6 +25,10 @@ gate computed from the layer's input (`output_gate`), query and key heads brough
 square of 1 after they turn, without a weight (`qk_norm="unit"`), and a sink whose score is a
 learned number per head (`sink="learned"`). Such a layer reads its input through one
 product (`input_width`), which layers side by side may share.
+
+Requests may have low-rank adapters beside the projections (`adapter_spots`): beside q, k, v (and
+the output gate), which are one product, and beside the output projection. A step in which a request has
+one runs the product, the adapters and the rotation one after the other.
 """
 from __future__ import annotations
 
@@ -35,7 +39,7 @@ import torch
 
 from ..registry import register_part
 from ..weights.source import TensorSpec
-from .base import CacheNeed, CallInfo, Mixer, Part, PositionEncoding, StepContext, WeightBinder
+from .base import AdapterSpot, CacheNeed, CallInfo, Mixer, Part, PositionEncoding, StepContext, WeightBinder
 
 
 class Attention(Mixer):
@@ -144,6 +148,25 @@ class Attention(Mixer):
         self.w_qkv: Optional[torch.Tensor] = None
         self.b_qkv: Optional[torch.Tensor] = None
         self.w_o: Optional[torch.Tensor] = None
+        inputs = [(key, width) for key, width in self._input_weights() if width]
+        self.spot_in = AdapterSpot(hidden, tuple((prefix + self.names[key], width) for key, width in inputs))
+        self.spot_out = AdapterSpot(heads * self.vdim, ((prefix + self.names["o"], hidden),))
+
+    def adapter_spots(self) -> List[AdapterSpot]:
+        return [self.spot_in, self.spot_out]
+
+    def add_input_adapters(self, ctx: StepContext, x, u) -> None:
+        self.spot_in.add(ctx, x, u)
+
+    def add_output_adapters(self, ctx: StepContext, rows, y) -> None:
+        self.spot_out.add(ctx, rows, y)
+
+    def _input_weights(self):
+        """The weights of the input product, in the order of its columns: (name's key, columns)."""
+        d = self.head_dim
+        return (("q", self.heads * d), ("k", self.kv_heads * d if self.own_kv else 0),
+                ("v", self.kv_heads * self.vdim if self.own_kv and self.values == "own" else 0),
+                ("g", self.heads * self.vdim if self.output_gate else 0))
 
     @property
     def qkv_width(self) -> int:
@@ -249,11 +272,9 @@ class Attention(Mixer):
     def bind_input(self, w: WeightBinder, rows: torch.Tensor) -> None:
         """The input product's weights into `rows` [input_width, hidden]: q, k, v (where values
         are projected), the gate's."""
-        p, d, n = self.prefix, self.head_dim, self.names
+        p, n = self.prefix, self.names
         at = 0
-        for key, width in (("q", self.heads * d), ("k", self.kv_heads * d),
-                           ("v", self.kv_heads * self.vdim if self.values == "own" else 0),
-                           ("g", self.heads * self.vdim if self.output_gate else 0)):
+        for key, width in self._input_weights():
             if width:
                 w.matrix_into(p + n[key], rows[at:at + width])
                 at += width
@@ -292,6 +313,7 @@ class Attention(Mixer):
                              f"its own, one without reads another's")
         u = ctx.empty((ctx.T, self.qkv_width))
         ops.linear(x, self.w_qkv, u)
+        self.spot_in.add(ctx, x, u)
         q = ctx.empty((ctx.T, self.heads * self.head_dim))
         ops.qkv_conv(u, self.w_conv, call.state, ctx, q, self.heads,
                      self.kv_heads if self.own_kv else 0, self.head_dim, self.vdim, cache["k"],
@@ -305,25 +327,31 @@ class Attention(Mixer):
                             attn, slopes=self.slopes, vdim=self.vdim, sink=self.sink)
         out = ctx.empty((ctx.T, self.hidden))
         ops.linear(attn, self.w_o, out)
+        self.spot_out.add(ctx, attn, out)
         return out
 
     def forward(self, ctx: StepContext, x, residual, call: CallInfo):
         if self.wide:
             u = ctx.empty((ctx.T, self.input_width()))
             ctx.ops.linear(x, self.w_qkv, u)
+            self.add_input_adapters(ctx, x, u)
             return self.forward_projected(ctx, u, call)
         if self.general:
             return self._forward_general(ctx, x, call)
         ops = ctx.ops
         cache = call.cache
         qkv = ctx.empty((ctx.T, self.qkv_width))
-        # the product, then bias, rotation of q and k, and the write of k, v into pages
-        ops.qkv_rope(x, self.w_qkv, self.b_qkv, qkv, ctx.positions, ctx.row_seq,
-                     self.position.table(), self.position.rot_dim, self.heads, self.kv_heads,
-                     self.head_dim, cache["k"], cache["v"], cache.block_table,
-                     cache.page_size, write_kv=call.writes_cache,
-                     interleaved=self.position.pairing == "interleaved",
-                     q_norm=self.q_norm, k_norm=self.k_norm, norm_eps=self.qk_norm_eps or 0.0)
+        # the product (what adapters add to it), then bias, rotation of q and k, and the write of k, v into pages
+        where = (ctx.positions, ctx.row_seq, self.position.table(), self.position.rot_dim, self.heads, self.kv_heads,
+                 self.head_dim, cache["k"], cache["v"], cache.block_table, cache.page_size)
+        how = dict(write_kv=call.writes_cache, interleaved=self.position.pairing == "interleaved",
+                   q_norm=self.q_norm, k_norm=self.k_norm, norm_eps=self.qk_norm_eps or 0.0)
+        if ctx.row_adapter is None:
+            ops.qkv_rope(x, self.w_qkv, self.b_qkv, qkv, *where, **how)
+        else:
+            ops.linear(x, self.w_qkv, qkv)
+            self.spot_in.add(ctx, x, qkv)
+            ops.rope_kv_write(qkv, self.b_qkv, *where, **how)
         attn = ctx.empty((ctx.T, self.heads * self.head_dim))
         ops.paged_attention(qkv, cache["k"], cache["v"], cache.block_table, ctx,
                             self.heads, self.kv_heads, self.head_dim,
@@ -331,6 +359,7 @@ class Attention(Mixer):
                             sink=self.sink)
         out = ctx.empty((ctx.T, self.hidden))
         ops.linear(attn, self.w_o, out)
+        self.spot_out.add(ctx, attn, out)
         return out
 
 

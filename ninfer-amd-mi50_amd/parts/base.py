@@ -136,6 +136,7 @@ class StepContext:
     all_decode: bool = False
     single_rows: int = 0          # the first single_rows requests bring one row each (rows 0 ..)
     portion_keys: int = 0         # cached positions of the requests behind them, this step's included (0: not said)
+    row_adapter: Optional[torch.Tensor] = None   # [T] number of each row's adapter, -1 for none; None: no row has one
     scratch: Dict[str, Any] = field(default_factory=dict)
 
     def empty(self, shape, dtype=None) -> torch.Tensor:
@@ -237,6 +238,33 @@ class NormedOutput:
     y: Any
 
 
+@dataclass
+class AdapterSpot:
+    """A product of a part beside which requests may have low-rank adapters: what it reads (`width` numbers a row) and
+    the checkpoint weights whose outputs lie side by side in its rows, each with its number of columns. `tables` holds
+    the adapters' factors once the engine has made room for them."""
+    width: int
+    weights: Tuple[Tuple[str, int], ...]
+    tables: Optional["AdapterTables"] = None
+
+    def add(self, ctx: "StepContext", x: torch.Tensor, out: torch.Tensor) -> None:
+        """What the adapters of the step's rows add to the product's rows `out` of x, in place."""
+        if ctx.row_adapter is not None and self.tables is not None:
+            t = self.tables
+            ctx.ops.adapter_add(x, t.a, t.b, t.scale, t.ranks, t.widths, ctx.row_adapter, out)
+
+
+@dataclass
+class AdapterTables:
+    """The factors of up to L adapters of rank R at one spot of S weights: a [L, S R, width], b [L, columns, R] in the
+    activation dtype, scale [L] (32-bit), ranks [L] (int32; 0: this adapter has nothing here)."""
+    a: torch.Tensor
+    b: torch.Tensor
+    scale: torch.Tensor
+    ranks: torch.Tensor
+    widths: Tuple[int, ...]
+
+
 def plain_rows(ctx: "StepContext", y):
     """What a part handed on as something that any part takes: a NormedSum, a SumRows or a
     NormedRows becomes rows, a ReadyRows nothing; everything else is handed back unchanged. (A NormedOutput is no
@@ -314,6 +342,13 @@ class Part:
 
     def children(self) -> List["Part"]:
         return []
+
+    def adapter_spots(self) -> List[AdapterSpot]:
+        """The products of this part beside which requests may have adapters."""
+        return []
+
+    def all_adapter_spots(self) -> List[AdapterSpot]:
+        return self.adapter_spots() + [s for c in self.children() for s in c.all_adapter_spots()]
 
     def max_positions(self) -> Optional[int]:
         """The most positions a request may have because of this part (a table of learned
@@ -413,8 +448,18 @@ class Mixer(Part):
         """The output product of what `mix_projected` returned."""
         raise NotImplementedError
 
+    def add_input_adapters(self, ctx: StepContext, x: torch.Tensor, u: torch.Tensor) -> None:
+        """What adapters add to the shared product's columns of this mixer: called with what `mix_projected` is about to
+        take, after the product."""
+
+    def add_output_adapters(self, ctx: StepContext, rows: torch.Tensor, y: torch.Tensor) -> None:
+        """... and to `y`, what `output` made of `rows`."""
+
     def forward_projected(self, ctx: StepContext, u: torch.Tensor, call: CallInfo, extra=None) -> torch.Tensor:
-        return self.output(ctx, self.mix_projected(ctx, u, call, extra))
+        rows = self.mix_projected(ctx, u, call, extra)
+        y = self.output(ctx, rows)
+        self.add_output_adapters(ctx, rows, y)
+        return y
 
     def forward(self, ctx: StepContext, x: torch.Tensor, residual: torch.Tensor,
                 call: CallInfo) -> Optional[torch.Tensor]:

@@ -77,6 +77,8 @@ class SideBySide(Mixer):
         with ops.together():
             ops.linear(x, self.w_in, u)
             extra_l, extra_r = self.left.input_extra(ctx, x), self.right.input_extra(ctx, x)
+        self.left.add_input_adapters(ctx, x, u[:, :a])
+        self.right.add_input_adapters(ctx, x, u[:, a:])
         to_left = self._call(call, self.left, 0)
         to_right = self._call(call, self.right, self.left.state_floats())
         if ops.wants_beside(ctx.T):
@@ -89,6 +91,8 @@ class SideBySide(Mixer):
             r = self.right.mix_projected(ctx, u[:, a:], to_right, extra_r)
             with ops.together():
                 y_l, y_r = self.left.output(ctx, l), self.right.output(ctx, r)
+            self.left.add_output_adapters(ctx, l, y_l)
+            self.right.add_output_adapters(ctx, r, y_r)
         if self.left_norm is None:
             return SumRows(y_l, self.left_factor, y_r, self.right_factor)
         return NormedSum(y_l, self.gain_l, y_r, self.gain_r, self.eps, self.factor)

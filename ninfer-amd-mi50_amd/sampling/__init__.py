@@ -1,4 +1,4 @@
 from .params import SamplingParams
-from .sampler import SampleRow, Sampler, fresh_seed, uniform
+from .sampler import SampleRow, Sampler, TokenLogprob, fresh_seed, uniform
 
-__all__ = ["SamplingParams", "SampleRow", "Sampler", "fresh_seed", "uniform"]
+__all__ = ["SamplingParams", "SampleRow", "Sampler", "TokenLogprob", "fresh_seed", "uniform"]

@@ -7,11 +7,16 @@ repetition penalty over prompt + generated tokens, greedy if temperature
 draw is a counter hash of (seed, request key, draw index), so a request's
 tokens do not depend on what it was batched with. Seed 0 means "not fixed":
 the request gets a seed from the operating system when it is added.
+
+Rows that ask for more than the reference's options (presence and frequency penalties, biases, a set of
+allowed tokens) have their logits changed before that, in one pass over a copy of the step's rows;
+their repetition penalty is then part of that pass.
 """
 from __future__ import annotations
 
 import os
 from array import array
+from dataclasses import dataclass
 from itertools import accumulate
 from operator import attrgetter
 from typing import Dict, Iterable, List, Optional, Sequence, Tuple
@@ -74,14 +79,14 @@ def fresh_seed() -> int:
 
 class History:
     """How often a request has seen each token (prompt + generated), for the
-    repetition penalty. Kept as two growing arrays (distinct tokens, counts), so
+    repetition penalty, and how often it has generated it. Kept as growing arrays (distinct tokens, counts), so
     that a step hands them to the device as they are: the work per generated
     token does not grow with the length of the history."""
 
     def __init__(self, tokens: Iterable[int] = ()):
         toks, counts = np.unique(np.asarray(list(tokens), dtype=np.int64), return_counts=True)
         n = int(toks.shape[0])
-        self._both = np.zeros((2, max(64, 2 * n)), np.int32)   # tokens, then counts
+        self._both = np.zeros((3, max(64, 2 * n)), np.int32)   # tokens, then counts, then those generated
         self._both[0, :n] = toks
         self._both[1, :n] = counts
         self._n = n
@@ -92,12 +97,12 @@ class History:
             self._where = {int(t): i for i, t in enumerate(self._both[0, :self._n])}
         i = self._where.get(token)
         if i is not None:
-            self._both[1, i] += 1
+            self._both[1:, i] += 1
             return
         if self._n == self._both.shape[1]:
             self._both = np.concatenate([self._both, np.zeros_like(self._both)], axis=1)
         self._both[0, self._n] = token
-        self._both[1, self._n] = 1
+        self._both[1:, self._n] = 1
         self._where[token] = self._n
         self._n += 1
 
@@ -107,6 +112,10 @@ class History:
 
     def both(self) -> np.ndarray:
         """`arrays` as the two rows of one view."""
+        return self._both[:2, :self._n]
+
+    def all(self) -> np.ndarray:
+        """The distinct tokens, their counts, and how many of these were generated (added one by one), as rows of one view."""
         return self._both[:, :self._n]
 
     def count(self, token: int) -> int:
@@ -119,15 +128,53 @@ class History:
 
 
 class SampleRow:
-    """What the sampler needs of one row: options, history counts, RNG stream."""
+    """What the sampler needs of one row: options, history counts, RNG stream, and which tokens may come (`allowed`:
+    words of `allowed_words`, or None for all)."""
 
-    def __init__(self, params: SamplingParams, history: History, key: int, draw: int, seed: int):
+    def __init__(self, params: SamplingParams, history: History, key: int, draw: int, seed: int,
+                 allowed: Optional[np.ndarray] = None):
         self.params = params
+        self.allowed = allowed
+        # (a change of logits beyond the repetition penalty, which the sampling kernels apply themselves)
+        self.changes = allowed is not None or bool(params.presence_penalty or params.frequency_penalty or params.logit_bias)
         self.history = history if isinstance(history, History) else History(
             t for t, c in dict(history).items() for _ in range(c))
         self.key = key
         self.draw = draw
         self.seed = seed
+
+
+def allowed_words(allowed, vocab: int) -> Optional[np.ndarray]:
+    """What may come next as words of 32 tokens (bit t % 32 of word t // 32). `allowed`: None (everything), an array of uint32,
+    which are these words already, or token ids. ValueError where nothing may come, or an id or the size is wrong."""
+    if allowed is None:
+        return None
+    n = (vocab + 31) // 32
+    if isinstance(allowed, np.ndarray) and allowed.dtype == np.uint32:
+        if allowed.shape != (n,):
+            raise ValueError(f"a mask of {vocab} tokens has {n} words, not {allowed.shape}")
+        words = allowed.copy()
+        if vocab % 32:
+            words[-1] &= np.uint32((1 << vocab % 32) - 1)
+    else:
+        ids = np.asarray(list(allowed), dtype=np.int64)
+        if ids.size and not (0 <= ids.min() and ids.max() < vocab):
+            raise ValueError(f"an allowed token is outside [0, {vocab})")
+        words = np.zeros(n, np.uint32)
+        np.bitwise_or.at(words, ids // 32, np.uint32(1) << (ids % 32).astype(np.uint32))
+    if not words.any():
+        raise ValueError("no token is allowed")
+    return words
+
+
+@dataclass
+class TokenLogprob:
+    """A token's log-probability under its row of logits, its place in the row's order (0: the most likely), and the best
+    tokens of the row with theirs."""
+    token: int
+    logprob: float
+    place: int
+    best: List[Tuple[int, float]]
 
 
 class Sampler:
@@ -150,8 +197,85 @@ class Sampler:
             slot = (buffer, buffer.numpy())
         return slot
 
+    def _upload(self, arrays: List[np.ndarray]) -> Tuple[List[torch.Tensor], Optional[tuple]]:
+        """Arrays of 32-bit numbers on the device, in one copy, and the pinned buffer that it is made out of: to be given back
+        (`_free`) once the stream has been waited for."""
+        sizes = [a.size for a in arrays]
+        n, slot = sum(sizes), None
+        if self.device.type == "cuda":
+            slot = pinned, packed = self._staged(n)
+        else:
+            packed = np.empty(n, np.int32)
+        np.concatenate([a.reshape(-1).view(np.int32) for a in arrays], out=packed[:n])
+        if slot is None:
+            flat = torch.from_numpy(packed)
+        else:
+            flat = torch.empty(n, dtype=torch.int32, device=self.device)
+            flat.copy_(pinned[:n], non_blocking=True)
+        return [t.view(torch.float32) if a.dtype == np.float32 else t for a, t in zip(arrays, flat.split(sizes))], slot
+
+    def adjusted(self, logits: torch.Tensor, rows: Sequence[SampleRow]) -> Tuple[torch.Tensor, Optional[tuple]]:
+        """The rows' logits as their requests ask for them (repetition penalty included, of rows that ask for more than it), in
+        a tensor of their own; and the buffer that `_upload` gives."""
+        r, vocab, f32, i32 = len(rows), logits.shape[1], np.float32, np.int32
+        none = History()
+        asked = [row.params if row.changes else None for row in rows]
+
+        def numbers(name, default):
+            return np.array([default if p is None else getattr(p, name) for p in asked], f32)
+
+        def offsets(sizes):
+            return np.array(list(accumulate(sizes, initial=0)), i32)
+
+        given = [("repetition", numbers("repetition_penalty", 1.0)), ("presence", numbers("presence_penalty", 0.0)),
+                 ("frequency", numbers("frequency_penalty", 0.0))]
+        histories = [row.history if p is not None and (p.repetition_penalty != 1.0 or p.presence_penalty or p.frequency_penalty)
+                     else none for row, p in zip(rows, asked)]
+        if any(len(h) for h in histories):
+            seen = np.concatenate([h.all() for h in histories], axis=1)
+            given += [("hist_offsets", offsets(map(len, histories))), ("hist_tokens", seen[0]), ("hist_counts", seen[1]),
+                      ("hist_generated", seen[2])]
+        biases = [(p.logit_bias or {}) if p is not None else {} for p in asked]
+        if any(biases):
+            given += [("bias_offsets", offsets(map(len, biases))),
+                      ("bias_tokens", np.array([int(t) for b in biases for t in b], i32)),
+                      ("bias_values", np.array([v for b in biases for v in b.values()], f32))]
+        masks = [row.allowed for row in rows if row.allowed is not None]
+        if masks:
+            number = iter(range(len(masks)))
+            given += [("masks", np.stack(masks)),
+                      ("mask_rows", np.array([-1 if row.allowed is None else next(number) for row in rows], i32))]
+        tensors, slot = self._upload([a for _, a in given])
+        kw = {name: t for (name, _), t in zip(given, tensors)}
+        if masks:
+            kw["masks"] = kw["masks"].view(len(masks), (vocab + 31) // 32)
+        out = torch.empty((r, vocab), dtype=torch.float32, device=logits.device)
+        self.ops.adjust_logits(logits, out, **kw)
+        return out, slot
+
+    def logprobs(self, logits: torch.Tensor, tokens: Sequence[int], top: int = 0) -> List[TokenLogprob]:
+        """The log-probabilities of one token per row of `logits` [R, vocab], and of each row's `top` best."""
+        slot = None
+        if len(tokens) == 0:
+            return []
+        (of,), slot = self._upload([np.asarray(tokens, np.int32)])
+        p, before, best, best_p = self.ops.token_logprobs(logits, of, top)
+        rows = zip(tokens, p.tolist(), before.tolist(), best.tolist(), best_p.tolist())
+        if slot is not None:
+            self._free.append(slot)   # (the results are there, so is the copy)
+        return [TokenLogprob(int(t), lp, n, list(zip(ids, lps))) for t, lp, n, ids, lps in rows]
+
     def sample(self, logits: torch.Tensor, rows: Sequence[SampleRow]) -> List[int]:
         """One token per row of `logits` [R, vocab]."""
+        if not any(row.changes for row in rows):
+            return self._sample(logits, rows)
+        logits, slot = self.adjusted(logits, rows)
+        tokens = self._sample(logits, rows)
+        if slot is not None:
+            self._free.append(slot)
+        return tokens
+
+    def _sample(self, logits: torch.Tensor, rows: Sequence[SampleRow]) -> List[int]:
         r = len(rows)
         assert logits.shape[0] == r
         # Everything the kernel needs of the rows travels in one array and one copy: four
@@ -159,6 +283,8 @@ class Sampler:
         # and counts. (Copies queue behind the step that makes the logits, one after the other:
         # every further one would add its latency to the step.)
         temps, tops, penalties, top_ks = zip(*map(_OPTIONS, (row.params for row in rows))) if r else ((),) * 4
+        # (rows whose logits were changed have had their penalty)
+        penalties = [1.0 if row.changes else penalty for row, penalty in zip(rows, penalties)]
         listed = [len(row.history) if penalty != 1.0 else 0 for row, penalty in zip(rows, penalties)]
         n_pen = sum(listed)
         o = 5 * r
