@@ -83,38 +83,55 @@ __device__ __forceinline__ Frag<T> load_frag(const T* row, int at, int n) {
   return f;
 }
 
-// The adapters of the 16 rows from t0 on: every wave goes through them in the order of their first rows.
+// The adapters of the 16 RT rows from t0 on: every wave goes through them in the order of their first rows.
+template <int RT>
 struct TileAdapters {
-  int mine;                 // lane i < 16: row t0 + i's adapter, -1 for none
+  int mine;                 // lane i < 16 RT: row t0 + i's adapter, -1 for none
+  int ranks;                // lane i < L: adapter i's rank (where there are up to 64; else asked for when it is needed)
   unsigned long long left;  // rows whose adapter has not been taken yet
   __device__ __forceinline__ TileAdapters(const AdapterArgs& a, int t0) {
     const int lane = threadIdx.x & 63;
-    mine = lane < 16 && t0 + lane < a.T ? a.row_adapter[t0 + lane] : -1;
+    mine = lane < 16 * RT && t0 + lane < a.T ? a.row_adapter[t0 + lane] : -1;
+    ranks = a.L <= 64 && lane < a.L ? a.ranks[lane] : 0;
     if (mine >= a.L || mine < 0) mine = -1;
     left = __ballot(mine >= 0);
   }
-  // The next adapter and the rows (bits) that have it.
-  __device__ __forceinline__ int next(unsigned& rows) {
+  // The next adapter, the rows (bits) that have it, and its rank.
+  __device__ __forceinline__ int next(const AdapterArgs& a, unsigned long long& rows, int& rank) {
     const int g = __builtin_amdgcn_readlane(mine, __ffsll(left) - 1);
-    rows = (unsigned)__ballot(mine == g);
-    left &= ~(unsigned long long)rows;
+    rows = __ballot(mine == g);
+    left &= ~rows;
+    rank = a.L <= 64 ? __builtin_amdgcn_readlane(ranks, g) : a.ranks[g];
+    rank = min(max(rank, 0), a.R);
     return g;
   }
 };
 
-template <typename T, int CT, bool VEC>
-__global__ __launch_bounds__(kShrinkWaves * 64) void adapter_shrink_kernel(const AdapterArgs a, int groups) {
-  __shared__ float part[kShrinkWaves][CT][64][4];
+// The work of a block: with `per` > 0 blocks that run on one XCD (block id mod 8) take neighbouring work, so that a
+// request's rows find its factors in that XCD's L2; -1 behind the last.
+__device__ __forceinline__ int work_of_block(int per, int total) {
+  const int b = per ? blockIdx.x % kXcds * per + blockIdx.x / kXcds : blockIdx.x;
+  return b < total ? b : -1;
+}
+
+// h of 16 RT rows and 16 CT columns.
+template <typename T, int RT, int CT, bool VEC>
+__global__ __launch_bounds__(kShrinkWaves * 64) void adapter_shrink_kernel(const AdapterArgs a, int groups, int per, int total) {
+  __shared__ float part[kShrinkWaves][RT * CT][64][4];
   constexpr int kLane = Frag<T>::kLane, kStep = 4 * kLane;
-  const int t0 = blockIdx.x / groups * 16, j0 = blockIdx.x % groups * (CT * 16);
+  const int b = work_of_block(per, total);
+  if (b < 0) return;
+  const int t0 = b / groups * (16 * RT), j0 = b % groups * (CT * 16);
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, quad = lane >> 4, C = a.S * a.R;
-  const T* xrow = (const T*)a.x + (int64_t)min(t0 + (lane & 15), a.T - 1) * a.ldx;
-  TileAdapters tile(a, t0);
+  const T* xrow[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) xrow[rt] = (const T*)a.x + (int64_t)min(t0 + rt * 16 + (lane & 15), a.T - 1) * a.ldx;
+  TileAdapters<RT> tile(a, t0);
   for (int pass = 0; tile.left; ++pass) {
-    unsigned rows;
-    const int g = tile.next(rows);
+    unsigned long long rows;
+    int rank;
+    const int g = tile.next(a, rows, rank);
     if (pass % gridDim.y != blockIdx.y) continue;
-    const int rank = min(max(a.ranks[g], 0), a.R);
     bool any = false;
     const T* arow[CT];
 #pragma unroll
@@ -124,42 +141,53 @@ __global__ __launch_bounds__(kShrinkWaves * 64) void adapter_shrink_kernel(const
       arow[ct] = (const T*)a.a + ((int64_t)g * C + min(j, C - 1)) * a.K;
     }
     if (!__ballot(any)) continue;
-    f32x4 acc[CT];
+    f32x4 acc[RT][CT];
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) acc[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) acc[rt][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
     // wave w takes the steps w, w + 8, ..
-    const int whole = VEC ? a.K / kStep : 0;
     int st = w;
     if constexpr (VEC) {
+      const int whole = a.K / kStep;
 #pragma unroll 4
       for (; st < whole; st += kShrinkWaves) {
         const int k = st * kStep + quad * kLane;
-        Frag<T> xf;
-        xf.v = *(const decltype(xf.v)*)(xrow + k);
+        Frag<T> xf[RT], af[CT];
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          Frag<T> af;
-          af.v = *(const decltype(af.v)*)(arow[ct] + k);
-          acc[ct] = Frag<T>::mma(xf, af, acc[ct]);
-        }
+        for (int rt = 0; rt < RT; ++rt) xf[rt].v = *(const decltype(xf[rt].v)*)(xrow[rt] + k);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) af[ct].v = *(const decltype(af[ct].v)*)(arow[ct] + k);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) acc[rt][ct] = Frag<T>::mma(xf[rt], af[ct], acc[rt][ct]);
       }
     }
     for (; st * kStep < a.K; st += kShrinkWaves) {
       const int k = st * kStep + quad * kLane;
-      const Frag<T> xf = load_frag<VEC>(xrow, k, a.K);
+      Frag<T> xf[RT];
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) acc[ct] = Frag<T>::mma(xf, load_frag<VEC>(arow[ct], k, a.K), acc[ct]);
+      for (int rt = 0; rt < RT; ++rt) xf[rt] = load_frag<VEC>(xrow[rt], k, a.K);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        const Frag<T> af = load_frag<VEC>(arow[ct], k, a.K);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) acc[rt][ct] = Frag<T>::mma(xf[rt], af, acc[rt][ct]);
+      }
     }
     __syncthreads();   // (the pass before has read its sums)
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) *(f32x4*)part[w][ct][lane] = acc[ct];
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) *(f32x4*)part[w][rt * CT + ct][lane] = acc[rt][ct];
     __syncthreads();
-    for (int o = threadIdx.x; o < CT * 256; o += kShrinkWaves * 64) {
-      const int ct = o >> 8, l = (o >> 2) & 63, row = (l >> 4) * 4 + (o & 3), j = j0 + ct * 16 + (l & 15);
+    for (int o = threadIdx.x; o < RT * CT * 256; o += kShrinkWaves * 64) {
+      const int f = o >> 8, l = (o >> 2) & 63, row = f / CT * 16 + (l >> 4) * 4 + (o & 3), j = j0 + f % CT * 16 + (l & 15);
       if (!(rows >> row & 1) || j >= C || j % a.R >= rank) continue;
       float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < kShrinkWaves; ++i) sum += part[i][ct][l][o & 3];
+      for (int i = 0; i < kShrinkWaves; ++i) sum += part[i][f][l][o & 3];
       a.h[(int64_t)(t0 + row) * C + j] = sum;
     }
   }
@@ -184,12 +212,19 @@ __device__ __forceinline__ void load_h(const float* row, int at, int n, Frag<bf1
   }
 }
 
-// Sixteen neighbouring columns of a row, the ones before `n` of them.
+// Sixteen neighbouring columns of a row, the ones before `n` of them; VEC: 16 bytes at a time.
 template <typename T>
 __device__ __forceinline__ void load_16(const T* p, int n, bool vec, float* f) {
+  constexpr int kEach = 16 / sizeof(T);
   if (vec && n >= 16) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) load_row<4>(p + 4 * i, f + 4 * i);
+    for (int i = 0; i < 16; i += kEach) {
+      const uint4 v = *(const uint4*)(p + i);
+      T e[kEach];
+      __builtin_memcpy(e, &v, 16);
+#pragma unroll
+      for (int c = 0; c < kEach; ++c) f[i + c] = to_f32(e[c]);
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 16; ++i) f[i] = i < n ? to_f32(p[i]) : 0.f;
@@ -197,9 +232,17 @@ __device__ __forceinline__ void load_16(const T* p, int n, bool vec, float* f) {
 }
 template <typename T>
 __device__ __forceinline__ void store_16(T* p, int n, bool vec, const float* f) {
+  constexpr int kEach = 16 / sizeof(T);
   if (vec && n >= 16) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) store_row<4>(p + 4 * i, f + 4 * i);
+    for (int i = 0; i < 16; i += kEach) {
+      T e[kEach];
+#pragma unroll
+      for (int c = 0; c < kEach; ++c) e[c] = from_f32<T>(f[i + c]);
+      uint4 v;
+      __builtin_memcpy(&v, e, 16);
+      *(uint4*)(p + i) = v;
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 16; ++i)
@@ -207,11 +250,15 @@ __device__ __forceinline__ void store_16(T* p, int n, bool vec, const float* f) 
   }
 }
 
-template <typename T, bool VEC>
-__global__ __launch_bounds__(kExpandWaves * 64) void adapter_expand_kernel(const AdapterArgs a, int groups, int blocks, bool vec_out) {
+// 64 columns a wave, 16 RT rows.
+template <typename T, int RT, bool VEC>
+__global__ __launch_bounds__(kExpandWaves * 64) void adapter_expand_kernel(const AdapterArgs a, int groups, int blocks, int per, int total,
+                                                                           bool vec_out) {
   constexpr int kLane = Frag<T>::kLane, kStep = 4 * kLane;
-  const int t0 = blockIdx.x / blocks * 16, lane = threadIdx.x & 63, quad = lane >> 4, m = lane & 15;
-  int group = blockIdx.x % blocks * kExpandWaves + (threadIdx.x >> 6);
+  const int b = work_of_block(per, total);
+  if (b < 0) return;
+  const int t0 = b / blocks * (16 * RT), lane = threadIdx.x & 63, quad = lane >> 4, m = lane & 15;
+  int group = b % blocks * kExpandWaves + (threadIdx.x >> 6);
   if (group >= groups) return;
   int s = 0;
   for (; s < a.S - 1; ++s) {
@@ -220,81 +267,111 @@ __global__ __launch_bounds__(kExpandWaves * 64) void adapter_expand_kernel(const
     group -= here;
   }
   const int c0 = a.first[s] + group * 64, end = a.first[s + 1];
-  const int c = c0 + quad * 16, n = end - c;   // this lane's columns of row t0 + m
-  const int t = min(t0 + m, a.T - 1), C = a.S * a.R;
-  const T* from = (const T*)a.base + t * a.ldb + c;
-  T* to = (T*)a.out + t * a.ldo + c;
-  const float* hrow = a.h + (int64_t)t * C + s * a.R;
-  TileAdapters tile(a, t0);
-  if (a.base != a.out && blockIdx.y == 0 && t0 + m < a.T && !(tile.left >> m & 1)) {
-    float f[16];
-    load_16(from, n, vec_out, f);
-    store_16(to, n, vec_out, f);
+  const int c = c0 + quad * 16, n = end - c, C = a.S * a.R;   // this lane's columns of row t0 + 16 rt + m
+  TileAdapters<RT> tile(a, t0);
+  if (a.base != a.out && blockIdx.y == 0) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int t = t0 + rt * 16 + m;
+      if (t < a.T && !(tile.left >> (rt * 16 + m) & 1)) {
+        float f[16];
+        load_16((const T*)a.base + t * a.ldb + c, n, vec_out, f);
+        store_16((T*)a.out + t * a.ldo + c, n, vec_out, f);
+      }
+    }
   }
   for (int pass = 0; tile.left; ++pass) {
-    unsigned rows;
-    const int g = tile.next(rows);
+    unsigned long long rows;
+    int rank;
+    const int g = tile.next(a, rows, rank);
     if (pass % gridDim.y != blockIdx.y) continue;
-    const bool mine = rows >> m & 1;
-    float f[16];
-    if (mine) load_16(from, n, vec_out, f);
-    const int rank = min(max(a.ranks[g], 0), a.R);
     const T* brow[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       brow[j] = (const T*)a.b + ((int64_t)g * a.N + min(c0 + (m >> 2) * 16 + j * 4 + (m & 3), end - 1)) * a.R;
-    f32x4 acc[4];
+    f32x4 acc[RT][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[rt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int k0 = 0; k0 < rank; k0 += kStep) {
       const int k = k0 + quad * kLane;
-      Frag<T> high, low;
-      load_h<VEC>(hrow, k, rank, high, low);
+      Frag<T> bf[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const Frag<T> bf = load_frag<VEC>(brow[j], k, rank);
-        acc[j] = Frag<T>::mma(bf, high, acc[j]);
-        if constexpr (sizeof(T) == 2) acc[j] = Frag<T>::mma(bf, low, acc[j]);
+      for (int j = 0; j < 4; ++j) bf[j] = load_frag<VEC>(brow[j], k, rank);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        if (RT > 1 && !(rows >> (rt * 16) & 0xffff)) continue;
+        Frag<T> high, low;
+        load_h<VEC>(a.h + (int64_t)min(t0 + rt * 16 + m, a.T - 1) * C + s * a.R, k, rank, high, low);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          acc[rt][j] = Frag<T>::mma(bf[j], high, acc[rt][j]);
+          if constexpr (sizeof(T) == 2) acc[rt][j] = Frag<T>::mma(bf[j], low, acc[rt][j]);
+        }
       }
     }
-    if (!mine) continue;
     const float scale = a.scale[g];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int rt = 0; rt < RT; ++rt) {
+      const int t = t0 + rt * 16 + m;
+      if (!(rows >> (rt * 16 + m) & 1)) continue;
+      float f[16];
+      load_16((const T*)a.base + t * a.ldb + c, n, vec_out, f);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) f[j * 4 + i] += scale * acc[j][i];
+      for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[j * 4 + i] += scale * acc[rt][j][i];
+      }
+      store_16((T*)a.out + t * a.ldo + c, n, vec_out, f);
     }
-    store_16(to, n, vec_out, f);
   }
+}
+
+// Blocks side by side for the adapters that a tile of rows may have, while the tiles are few; one goes through them all where they
+// are many.
+static int side_by_side(const AdapterArgs& a, long long blocks, int rows) {
+  const int most = std::min(std::min(rows, a.T), a.L);
+  return (int)std::max(1ll, std::min<long long>(most, 4ll * device_cu_count() / blocks));
+}
+
+template <typename T, int RT, int CT>
+static void shrink(const AdapterArgs& a, hipStream_t stream) {
+  constexpr int kLane = Frag<T>::kLane;
+  const int groups = (a.S * a.R + CT * 16 - 1) / (CT * 16), total = (a.T + 16 * RT - 1) / (16 * RT) * groups;
+  const int per = RT > 1 ? (total + kXcds - 1) / kXcds : 0;
+  const dim3 grid(per ? per * kXcds : total, side_by_side(a, total, 16 * RT));
+  const bool vec = (uintptr_t)a.x % 16 == 0 && (uintptr_t)a.a % 16 == 0 && a.K % kLane == 0 && a.ldx % kLane == 0;
+  if (vec) adapter_shrink_kernel<T, RT, CT, true><<<grid, kShrinkWaves * 64, 0, stream>>>(a, groups, per, total);
+  else adapter_shrink_kernel<T, RT, CT, false><<<grid, kShrinkWaves * 64, 0, stream>>>(a, groups, per, total);
+}
+
+template <typename T, int RT>
+static void expand(const AdapterArgs& a, hipStream_t stream) {
+  constexpr int kLane = Frag<T>::kLane;
+  int groups = 0;
+  bool vec_out = (uintptr_t)a.out % 16 == 0 && (uintptr_t)a.base % 16 == 0 && a.ldo * sizeof(T) % 16 == 0 && a.ldb * sizeof(T) % 16 == 0;
+  for (int s = 0; s < a.S; ++s) {
+    groups += (a.first[s + 1] - a.first[s] + 63) / 64;
+    vec_out &= a.first[s] * sizeof(T) % 16 == 0;
+  }
+  const int blocks = (groups + kExpandWaves - 1) / kExpandWaves, total = (a.T + 16 * RT - 1) / (16 * RT) * blocks;
+  const int per = RT > 1 ? (total + kXcds - 1) / kXcds : 0;
+  const dim3 grid(per ? per * kXcds : total, side_by_side(a, total, 16 * RT));
+  const bool vec = (uintptr_t)a.b % 16 == 0 && a.R % kLane == 0;
+  if (vec) adapter_expand_kernel<T, RT, true><<<grid, kExpandWaves * 64, 0, stream>>>(a, groups, blocks, per, total, vec_out);
+  else adapter_expand_kernel<T, RT, false><<<grid, kExpandWaves * 64, 0, stream>>>(a, groups, blocks, per, total, vec_out);
 }
 
 template <typename T>
 static void launch(const AdapterArgs& a, hipStream_t stream) {
-  constexpr int kLane = Frag<T>::kLane;
-  const int tiles = (a.T + 15) / 16, C = a.S * a.R, cus = device_cu_count();
-  // Blocks of 64 columns share a tile of x between four products; blocks of 16 are more, where there are too few to fill the GPU.
-  const bool wide = (long long)tiles * ((C + 63) / 64) >= cus;
-  const int groups = wide ? (C + 63) / 64 : (C + 15) / 16;
-  // A block for each adapter that a tile may have, while the tiles are few; one goes through them all where they are many.
-  const int most = std::min(std::min(16, a.T), a.L);
-  auto side_by_side = [&](long long blocks) { return (int)std::max(1ll, std::min<long long>(most, 8ll * cus / blocks)); };
-  const bool vec = (uintptr_t)a.x % 16 == 0 && (uintptr_t)a.a % 16 == 0 && a.K % kLane == 0 && a.ldx % kLane == 0;
-  const dim3 grid(tiles * groups, side_by_side((long long)tiles * groups));
-  if (wide && vec) adapter_shrink_kernel<T, 4, true><<<grid, kShrinkWaves * 64, 0, stream>>>(a, groups);
-  if (wide && !vec) adapter_shrink_kernel<T, 4, false><<<grid, kShrinkWaves * 64, 0, stream>>>(a, groups);
-  if (!wide && vec) adapter_shrink_kernel<T, 1, true><<<grid, kShrinkWaves * 64, 0, stream>>>(a, groups);
-  if (!wide && !vec) adapter_shrink_kernel<T, 1, false><<<grid, kShrinkWaves * 64, 0, stream>>>(a, groups);
-  int sets = 0;
-  bool vec_out = (uintptr_t)a.out % 16 == 0 && (uintptr_t)a.base % 16 == 0 && a.ldo % 4 == 0 && a.ldb % 4 == 0;
-  for (int s = 0; s < a.S; ++s) {
-    sets += (a.first[s + 1] - a.first[s] + 63) / 64;
-    vec_out &= a.first[s] % 4 == 0;
+  if (a.T >= 512) {
+    shrink<T, 2, 4>(a, stream);
+    expand<T, 4>(a, stream);
+  } else {
+    shrink<T, 1, 1>(a, stream);
+    expand<T, 1>(a, stream);
   }
-  const int blocks = (sets + kExpandWaves - 1) / kExpandWaves;
-  const dim3 egrid(tiles * blocks, side_by_side((long long)tiles * blocks));
-  const bool evec = (uintptr_t)a.b % 16 == 0 && a.R % kLane == 0;
-  if (evec) adapter_expand_kernel<T, true><<<egrid, kExpandWaves * 64, 0, stream>>>(a, sets, blocks, vec_out);
-  else adapter_expand_kernel<T, false><<<egrid, kExpandWaves * 64, 0, stream>>>(a, sets, blocks, vec_out);
 }
 
 }  // namespace ninfer

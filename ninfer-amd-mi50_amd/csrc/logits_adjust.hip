@@ -30,8 +30,8 @@ struct AdjustArgs {
   int R, V, n_hist, n_bias, n_masks, vec;
 };
 
-constexpr int kAdjustThreads = 256;
-constexpr int kAdjustQuads = 4;   // groups of 4 logits a thread holds
+constexpr int kAdjustThreads = 512;
+constexpr int kAdjustQuads = 2;   // groups of 4 logits a thread holds
 constexpr int kAdjustPart = kAdjustThreads * kAdjustQuads * 4;
 constexpr int kAdjustLists = 8;   // list entries a thread has on their way at a time
 
@@ -44,31 +44,88 @@ __device__ __forceinline__ float penalised(float l, float p, unsigned count) {
   return (float)(l > 0.f ? (double)l / power : (double)l * power);
 }
 
-// Calls f(entry) for the entries [first, end) whose token lies in [t0, t0 + n).
-template <typename F>
-__device__ __forceinline__ void for_tokens_of_part(const int* tokens, int first, int end, int t0, int n, F f) {
-  for (int e0 = first + (int)threadIdx.x; e0 < end; e0 += kAdjustLists * kAdjustThreads) {
-    int t[kAdjustLists];
+struct AdjustLds {
+  // By token of the part: first what the list's entries say of it (0: nothing), then kListed and a 32-bit float.
+  unsigned long long of[kAdjustPart];
+  // The tokens of the part that stand in the list, as many as leave room for four blocks' memory on a CU; any further ones are
+  // found in `of`.
+  unsigned short listed[kAdjustPart - 4];
+  int n_listed;
+};
+static_assert(sizeof(AdjustLds) <= 40960, "four blocks to a CU");
+constexpr unsigned long long kListed = 1ull << 63;
+
+// One list of the row, entries [first, end): `note(entry, token)` puts an entry of the part into l.of and says whether it is
+// its token's first; `value(token, what l.of has)` makes a float of that; `put(logit, float)` goes over the listed tokens' logits.
+// The values are made by as many threads as tokens are listed: as a branch over the logits that a thread holds, nearly every wave would
+// run a power and a quotient in 64 bits for each of them (64 rows of 151,936 tokens and 2,500 entries 37 us so).
+template <typename Note, typename Value, typename Put>
+__device__ __forceinline__ bool apply_list(AdjustLds& l, const int* tokens, int first, int end, int t0, int n,
+                                           float (&v)[kAdjustQuads][4], Note note, Value value, Put put) {
+  constexpr int kMost = kAdjustPart - 4;
+  const int tid = threadIdx.x;
+  int t[kAdjustLists];
+  auto load = [&](int e0) {
 #pragma unroll
-    for (int u = 0; u < kAdjustLists; ++u) {
-      const int e = e0 + u * kAdjustThreads;
-      t[u] = tokens[e < end ? e : end - 1];
-    }
+    for (int u = 0; u < kAdjustLists; ++u) t[u] = tokens[min(e0 + u * kAdjustThreads, end - 1)];
+  };
+  load(first + tid);
+  __syncthreads();   // (the list before has been put)
+#pragma unroll
+  for (int i = 0; i < kAdjustPart / kAdjustThreads; ++i) l.of[i * kAdjustThreads + tid] = 0;
+  if (tid == 0) l.n_listed = 0;
+  __syncthreads();
+  for (int e0 = first + tid; e0 < end; e0 += kAdjustLists * kAdjustThreads) {
+    if (e0 != first + tid) load(e0);
 #pragma unroll
     for (int u = 0; u < kAdjustLists; ++u) {
       const int e = e0 + u * kAdjustThreads;
       const unsigned at = (unsigned)t[u] - (unsigned)t0;   // (ids outside the vocabulary fall outside every part)
-      if (e < end && at < (unsigned)n) f(e, (int)at);
+      if (e < end && at < (unsigned)n && note(e, (int)at)) {
+        const int i = atomicAdd(&l.n_listed, 1);
+        if (i < kMost) l.listed[i] = (unsigned short)at;
+      }
     }
   }
+  __syncthreads();
+  const int listed = l.n_listed;
+  for (int i = tid; i < min(listed, kMost); i += kAdjustThreads) {
+    const int at = l.listed[i];
+    l.of[at] = kListed | __float_as_uint(value(at, l.of[at]));
+  }
+  __syncthreads();
+  if (listed > kMost) {
+    for (int at = tid; at < kAdjustPart; at += kAdjustThreads)
+      if (l.of[at] && !(l.of[at] & kListed)) l.of[at] = kListed | __float_as_uint(value(at, l.of[at]));
+    __syncthreads();
+  }
+  if (listed) {
+#pragma unroll
+    for (int u = 0; u < kAdjustQuads; ++u) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const unsigned long long x = l.of[(u * kAdjustThreads + tid) * 4 + c];
+        if (x) put(v[u][c], __uint_as_float((unsigned)x));
+      }
+    }
+  }
+  return listed > 0;
 }
 
 __global__ __launch_bounds__(kAdjustThreads) void adjust_logits_kernel(const AdjustArgs a, int parts) {
-  __shared__ unsigned long long seen[kAdjustPart];   // counts: all in the lower half, generated ones in the upper
+  __shared__ AdjustLds l;
   const int r = blockIdx.x / parts, t0 = (blockIdx.x % parts) * kAdjustPart, tid = threadIdx.x;
   const int n = min(kAdjustPart, a.V - t0);
   const float* row = a.logits + r * a.ld + t0;
   float* to = a.out + r * a.ldo + t0;
+
+  // (everything that says where to look next is on its way at once)
+  int h0 = 0, h1 = 0, b0 = 0, b1 = 0, m = -1;
+  if (a.hist_offsets) h0 = a.hist_offsets[r], h1 = a.hist_offsets[r + 1];
+  if (a.bias_offsets) b0 = a.bias_offsets[r], b1 = a.bias_offsets[r + 1];
+  if (a.mask_rows) m = a.mask_rows[r];
+  const float rp = a.repetition ? a.repetition[r] : 1.f;
+  const float freq = a.frequency ? a.frequency[r] : 0.f, pres = a.presence ? a.presence[r] : 0.f;
 
   float v[kAdjustQuads][4];
 #pragma unroll
@@ -81,81 +138,50 @@ __global__ __launch_bounds__(kAdjustThreads) void adjust_logits_kernel(const Adj
       for (int c = 0; c < 4; ++c) v[u][c] = i + c < n ? row[i + c] : 0.f;
     }
   }
-
-  const float rp = a.repetition ? a.repetition[r] : 1.f;
-  const float freq = a.frequency ? a.frequency[r] : 0.f, pres = a.presence ? a.presence[r] : 0.f;
-  bool changed = a.out != a.logits;
-  int first = 0, end = 0;
-  if (a.hist_offsets && (rp != 1.f || freq != 0.f || pres != 0.f)) {
-    first = max(a.hist_offsets[r], 0);
-    end = min(a.hist_offsets[r + 1], a.n_hist);
-  }
-  if (end > first) {
-    for (int i = tid; i < kAdjustPart; i += kAdjustThreads) seen[i] = 0;
-    __syncthreads();
-    for_tokens_of_part(a.hist_tokens, first, end, t0, n, [&](int e, int at) {
-      const unsigned c = max(a.hist_counts[e], 0), g = a.hist_generated ? max(a.hist_generated[e], 0) : 0;
-      atomicAdd(&seen[at], (unsigned long long)g << 32 | c);
-    });
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < kAdjustQuads; ++u) {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const unsigned long long s = seen[(u * kAdjustThreads + tid) * 4 + c];
-        if (s == 0) continue;
-        changed = true;
-        float x = v[u][c];
-        if (rp != 1.f) x = penalised(x, rp, (unsigned)s);
-        const unsigned g = (unsigned)(s >> 32);
-        if (g) x = x - freq * (float)g - pres;
-        v[u][c] = x;
-      }
-    }
-  }
-  first = end = 0;
-  if (a.bias_offsets) {
-    first = max(a.bias_offsets[r], 0);
-    end = min(a.bias_offsets[r + 1], a.n_bias);
-  }
-  if (end > first) {
-    unsigned* last = (unsigned*)seen;   // 1 + the list's last entry for the token
-    __syncthreads();
-    for (int i = tid; i < kAdjustPart; i += kAdjustThreads) last[i] = 0;
-    __syncthreads();
-    for_tokens_of_part(a.bias_tokens, first, end, t0, n,
-                       [&](int e, int at) { atomicMax(&last[at], (unsigned)(e - first) + 1u); });
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < kAdjustQuads; ++u) {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const unsigned at = last[(u * kAdjustThreads + tid) * 4 + c];
-        if (at) {
-          v[u][c] += a.bias_values[first + at - 1];
-          changed = true;
-        }
-      }
-    }
-  }
-  const int m = a.mask_rows ? a.mask_rows[r] : -1;
-  if (m >= 0 && m < a.n_masks) {
+  const bool masked = m >= 0 && m < a.n_masks;
+  uint32_t bits[kAdjustQuads];
+  if (masked) {
     const uint32_t* words = a.masks + (int64_t)m * ((a.V + 31) / 32);
 #pragma unroll
     for (int u = 0; u < kAdjustQuads; ++u) {
-      const int i = (u * kAdjustThreads + tid) * 4;
-      if (i >= n) continue;
-      const uint32_t bits = words[(t0 + i) >> 5] >> ((t0 + i) & 31);
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (!(bits >> c & 1)) v[u][c] = -INFINITY;
+      const int i = t0 + min((u * kAdjustThreads + tid) * 4, n - 1);
+      bits[u] = words[i >> 5] >> (i & 28);
     }
-    changed = true;
+  }
+
+  bool changed = masked || a.out != a.logits;
+  h0 = max(h0, 0), h1 = min(h1, a.n_hist), b0 = max(b0, 0), b1 = min(b1, a.n_bias);
+  if (h1 > h0 && (rp != 1.f || freq != 0.f || pres != 0.f)) {
+    changed |= apply_list(
+        l, a.hist_tokens, h0, h1, t0, n, v,
+        [&](int e, int at) {
+          const unsigned c = max(a.hist_counts[e], 0), g = a.hist_generated ? max(a.hist_generated[e], 0) : 0;
+          return (c || g) && atomicAdd(&l.of[at], (unsigned long long)g << 32 | c) == 0;
+        },
+        [&](int at, unsigned long long counts) {
+          float x = row[at];
+          if (rp != 1.f) x = penalised(x, rp, (unsigned)counts);
+          const unsigned g = (unsigned)(counts >> 32);
+          return g ? x - freq * (float)g - pres : x;
+        },
+        [](float& logit, float x) { logit = x; });
+  }
+  if (b1 > b0) {
+    changed |= apply_list(
+        l, a.bias_tokens, b0, b1, t0, n, v,
+        [&](int e, int at) { return atomicMax(&l.of[at], (unsigned long long)(e - b0) + 1) == 0; },
+        [&](int, unsigned long long last) { return a.bias_values[b0 + (int)last - 1]; },
+        [](float& logit, float x) { logit += x; });
   }
   if (!changed) return;
 #pragma unroll
   for (int u = 0; u < kAdjustQuads; ++u) {
     const int i = (u * kAdjustThreads + tid) * 4;
+    if (masked) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (!(bits[u] >> c & 1)) v[u][c] = -INFINITY;
+    }
     if (a.vec && i + 4 <= n) {
       store_row<4>(to + i, v[u]);
     } else {

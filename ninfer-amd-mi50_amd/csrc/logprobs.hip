@@ -45,6 +45,7 @@ struct LogprobArgs {
 // The order of tokens: NaN behind everything.
 __device__ __forceinline__ uint32_t token_key(float v) { return v != v ? 0u : ordered_key(v); }
 
+// exp(v - m) for v <= m, as it goes into a sum; tokens at an infinite maximum count 1.
 __device__ __forceinline__ float exp_above(float v, float m) { return v == m ? 1.f : __expf(v - m); }
 
 __global__ __launch_bounds__(kLpThreads) void logprob_parts_kernel(const LogprobArgs a, int parts) {
@@ -53,44 +54,70 @@ __global__ __launch_bounds__(kLpThreads) void logprob_parts_kernel(const Logprob
   const int r = blockIdx.x / parts, part = blockIdx.x % parts, t0 = part * kLpPart, tid = threadIdx.x;
   const int n = min(kLpPart, a.V - t0), lane = tid & 63, w = tid >> 6;
   const float* row = a.logits + r * a.ld;
+  const int token = a.tokens ? a.tokens[r] : -1;
+  const bool asked = token >= 0 && token < a.V, whole = n == kLpPart;
   float v[kLpQuads][4];
 #pragma unroll
   for (int u = 0; u < kLpQuads; ++u) {
     const int i = (u * kLpThreads + tid) * 4;
-    if (a.vec && i + 4 <= n) {
+    if (a.vec && (whole || i + 4 <= n)) {
       load_row<4>(row + t0 + i, v[u]);
     } else {
 #pragma unroll
       for (int c = 0; c < 4; ++c) v[u][c] = i + c < n ? row[t0 + i + c] : -INFINITY;
     }
   }
-  const int token = a.tokens ? a.tokens[r] : -1;
-  const bool asked = token >= 0 && token < a.V;
-  const uint32_t mine = asked ? token_key(row[token]) : 0;
+  const float mine = asked ? row[token] : 0.f;
   float m = -INFINITY;
-  uint32_t most = 0;
-  int count = 0;
 #pragma unroll
-  for (int u = 0; u < kLpQuads; ++u) {
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int i = (u * kLpThreads + tid) * 4 + c;
-      const uint32_t k = i < n ? token_key(v[u][c]) : 0;
-      most = max(most, k);
-      count += i < n && (k > mine || (k == mine && t0 + i < token));
-      m = fmaxf(m, v[u][c]);
-    }
-  }
-  if (a.top) a.keys[((int64_t)r * parts + part) * kLpThreads + tid] = most;
+  for (int u = 0; u < kLpQuads; ++u) m = fmaxf(fmaxf(m, fmaxf(v[u][0], v[u][1])), fmaxf(v[u][2], v[u][3]));
+  // (a thread of nothing but NaN has the key of -inf, which its logits do not reach: the second launch notices)
+  if (a.top) a.keys[((int64_t)r * parts + part) * kLpThreads + tid] = ordered_key(m);
   m = wave_max(m);
   if (lane == 0) red_m[w] = m;
+
+  // What stands before the token: in parts before its own, logits as large as its own; in those behind it, larger ones.
+  int count = 0;
+  if (!asked) {
+  } else if (mine == mine && token >= t0 + kLpPart) {
+#pragma unroll
+    for (int u = 0; u < kLpQuads; ++u) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) count += v[u][c] >= mine;
+    }
+  } else if (mine == mine && token < t0) {
+#pragma unroll
+    for (int u = 0; u < kLpQuads; ++u) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) count += v[u][c] > mine;
+    }
+  } else {
+    const uint32_t key = token_key(mine);
+#pragma unroll
+    for (int u = 0; u < kLpQuads; ++u) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int i = (u * kLpThreads + tid) * 4 + c;
+        const uint32_t k = token_key(v[u][c]);
+        count += i < n && (k > key || (k == key && t0 + i < token));
+      }
+    }
+  }
   __syncthreads();
   m = fmaxf(fmaxf(red_m[0], red_m[1]), fmaxf(red_m[2], red_m[3]));
   float s = 0.f;
+  if (fabsf(m) < INFINITY) {
 #pragma unroll
-  for (int u = 0; u < kLpQuads; ++u) {
+    for (int u = 0; u < kLpQuads; ++u) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) s += exp_above(v[u][c], m);
+      for (int c = 0; c < 4; ++c) s += __expf(v[u][c] - m);
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < kLpQuads; ++u) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s += exp_above(v[u][c], m);
+    }
   }
   s = wave_sum(s);
 #pragma unroll
@@ -136,18 +163,36 @@ __device__ void best_by_turns(const LogprobArgs& a, const float* row, LpLds& l) 
   __syncthreads();
 }
 
-// Joins a row's parts; with TOP also its best tokens. Without, a block is one wave.
+// The logit of a key (+0 for -0; a key of NaN is asked for only in rows whose log-probabilities are all NaN).
+__device__ __forceinline__ float logit_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
+
+// Joins a row's parts; with TOP also its best tokens. Without, a block is one wave. What the second part of the work waits for,
+// one load after the other, is its time (8 us for one row of 151,936 tokens): the parts are joined by the last wave while the
+// others look for the bound, and keys are held from one look to the next.
 template <bool TOP>
 __global__ __launch_bounds__(TOP ? kLpJoinThreads : 64) void logprob_join_kernel(const LogprobArgs a, int parts) {
   __shared__ typename std::conditional<TOP, LpLds, int>::type lds;
+  constexpr int kHeld = 16;   // keys a thread holds: of rows of up to 262,144 tokens all
   const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   const float* row = a.logits + r * a.ld;
   const int64_t base = (int64_t)r * parts;
-  float m = -INFINITY, s = 0.f, log_sum = 0.f;
   auto log_p = [](float v, float m, float log_sum) {   // (a NaN among the logits is one in log_sum)
     return log_sum != log_sum ? log_sum : m == -INFINITY ? m : (v == m ? 0.f : v - m) - log_sum;
   };
-  if (tid < 64) {
+  const int n = parts * kLpThreads;
+  uint32_t held[kHeld];
+  if constexpr (TOP) {
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) {
+      const int i = tid + u * kLpJoinThreads;
+      held[u] = i < n ? a.keys[base * kLpThreads + i] : 0;
+    }
+  }
+  if (tid >= (TOP ? kLpJoinThreads - 64 : 0)) {
+    const int token = a.tokens ? a.tokens[r] : -1;
+    const bool asked = token >= 0 && token < a.V;
+    const float mine = asked ? row[token] : 0.f;
+    float m = -INFINITY, s = 0.f;
     int count = 0;
     for (int p = lane; p < parts; p += 64) m = fmaxf(m, a.sums[base + p].x);
     m = wave_max(m);
@@ -159,24 +204,27 @@ __global__ __launch_bounds__(TOP ? kLpJoinThreads : 64) void logprob_join_kernel
     s = wave_sum(s);
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) count += __shfl_xor(count, off, 64);
-    log_sum = logf(s);
-    if (lane == 0 && a.tokens) {
-      const int token = a.tokens[r];
-      const bool asked = token >= 0 && token < a.V;
-      a.logprob[r] = asked ? log_p(row[token], m, log_sum) : __builtin_nanf("");
-      a.before[r] = asked ? count : -1;
+    const float log_sum = logf(s);
+    if (lane == 0) {
+      if (a.tokens) {
+        a.logprob[r] = asked ? log_p(mine, m, log_sum) : __builtin_nanf("");
+        a.before[r] = asked ? count : -1;
+      }
+      if constexpr (TOP) lds.max = m, lds.log_sum = log_sum;
     }
   }
   if constexpr (TOP) {
     LpLds& l = lds;
-    if (tid == 0) l.max = m, l.log_sum = log_sum, l.segments = 0, l.n_found = 0;
+    if (tid == 0) l.segments = 0, l.n_found = 0;
     const uint32_t* keys = a.keys + base * kLpThreads;
-    const int n = parts * kLpThreads;
     uint32_t most = 0;
-    for (int i = tid; i < n; i += kLpJoinThreads) most = max(most, keys[i]);
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) most = max(most, held[u]);
+    for (int i = tid + kHeld * kLpJoinThreads; i < n; i += kLpJoinThreads) most = max(most, keys[i]);
     l.group[tid >> 6][lane] = most;
     __syncthreads();
     if (tid < 64) {
+#pragma unroll
       for (int i = 0; i < kLpJoinThreads / 64; ++i) most = max(most, l.group[i][lane]);
       int place = 0;
 #pragma unroll
@@ -188,12 +236,15 @@ __global__ __launch_bounds__(TOP ? kLpJoinThreads : 64) void logprob_join_kernel
     }
     __syncthreads();
     const uint32_t bound = l.bound;
-    for (int i = tid; i < n; i += kLpJoinThreads) {
-      if (keys[i] >= bound) {
+    auto list = [&](int i, uint32_t key) {
+      if (key >= bound && i < n) {
         const int at = atomicAdd(&l.segments, 1);
         if (at < kLpSegments) l.segment[at] = i;
       }
-    }
+    };
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) list(tid + u * kLpJoinThreads, held[u]);
+    for (int i = tid + kHeld * kLpJoinThreads; i < n; i += kLpJoinThreads) list(i, keys[i]);
     __syncthreads();
     const int segments = l.segments;
     if (segments <= kLpSegments) {
@@ -211,8 +262,7 @@ __global__ __launch_bounds__(TOP ? kLpJoinThreads : 64) void logprob_join_kernel
     }
     __syncthreads();
     const int found = l.n_found;
-    // (the bound may be a group without tokens, whose key no token of the row reaches from below: then all are found)
-    if (segments > kLpSegments || found > kLpFound) {
+    if (segments > kLpSegments || found > kLpFound || found < a.top) {
       best_by_turns(a, row, l);
     } else {
       for (int j = tid; j < found; j += kLpJoinThreads) {
@@ -224,9 +274,9 @@ __global__ __launch_bounds__(TOP ? kLpJoinThreads : 64) void logprob_join_kernel
       __syncthreads();
     }
     if (tid < a.top) {
-      const int i = (int)~(uint32_t)l.best[tid];
-      a.best[(int64_t)r * a.top + tid] = i;
-      a.best_logprob[(int64_t)r * a.top + tid] = log_p(row[i], l.max, l.log_sum);
+      const unsigned long long k = l.best[tid];
+      a.best[(int64_t)r * a.top + tid] = (int)~(uint32_t)k;
+      a.best_logprob[(int64_t)r * a.top + tid] = log_p(logit_of((uint32_t)(k >> 32)), l.max, l.log_sum);
     }
   }
 }

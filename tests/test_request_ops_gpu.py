@@ -290,6 +290,19 @@ def test_adjust_offsets_that_leave_the_lists_read_nothing(ops):
     assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("vocab", [4092, 4093, 4096, 9000])
+def test_adjust_lists_of_every_token(ops, vocab):
+    rows = 2
+    c = make_adjust(rows, vocab, 5)
+    order = random.Random(1).sample(range(vocab), vocab)
+    c["histories"] = [[(t, 1 + t % 3, t % 2) for t in order], []]
+    c["biases"] = [[], [(t, float(t % 17)) for t in order]]
+    logits = torch.randn(rows, vocab, device="cuda")
+    want, room = rc.adjusted(logits, **rounded(c))
+    ops.adjust_logits(logits, **on_gpu(c))
+    rc.close(logits, want, room)
+
+
 def test_adjust_refusals(ops):
     from ninfer_amd.kernels.ops import KernelError
     logits, one = torch.zeros(2, 64, device="cuda"), f32([1.0, 1.0])
@@ -365,6 +378,19 @@ def test_logprobs_of_infinities_and_nan(ops):
     assert math.isnan(p[3]) and before[3] == 4 and best[3] == [0, 1, 2]
     assert best[4][:2] == [10, 20] and before[4] == 1
     assert p[5] == 0.0 and best[5] == [4321, 0, 1] and bp[5] == [0.0, -INF, -INF]
+
+
+def test_logprobs_of_a_row_with_many_nan(ops):
+    # whole threads' logits and whole groups of them are NaN, and fewer than `top` are not
+    x = torch.full((3, 9000), NAN, device="cuda")
+    x[0, 100:120] = torch.arange(20.0)
+    x[1, ::64] = torch.randn(141, device="cuda")
+    x[2, 4096:] = torch.randn(4904, device="cuda")
+    p, before, best, _ = ops.token_logprobs(x, i32([119, 64, 5000]), 40)
+    for r in range(3):
+        key = torch.where(x[r].isnan(), torch.full_like(x[r], -INF), x[r]).cpu()
+        assert best[r].tolist() == torch.sort(key, descending=True, stable=True).indices[:40].tolist()
+    assert before[0] == 0 and p.isnan().all()
 
 
 @pytest.mark.parametrize("shift,pad", [(0, 3), (1, 3), (4, 4)])
