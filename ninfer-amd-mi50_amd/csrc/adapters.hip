@@ -6,18 +6,17 @@
 //   out[t, c] = base[t, c] + scale[g] sum_i B[g, c, i] h[t, s(c), i]
 //
 // Two launches: all slices' h, kept in 32 bits (scratch [T, S R]), then the columns. Both give a block
-// tiles of 16 rows on the matrix units, whatever adapters these rows have: the block takes the tile's
-// adapters one after the other, the rows of others ride along unwritten. Rows of a request are
-// neighbours, so a tile of a prompt's portion has one adapter, as a rule. In a step of single rows it may
-// have up to 16: these then go to blocks of their own (grid.z), side by side. The rows need no order
-// and the host no list of groups, so that a captured step serves whatever requests come.
+// tiles of 16 or 32 rows on the matrix units, whatever adapters these rows have: the products of a tile and
+// one of its adapters are a block's work, the rows of others ride along unwritten. Rows of a request are
+// neighbours, so a tile of a prompt's portion has one adapter, as a rule; a tile of single rows may have as
+// many as rows. A step of few rows has blocks for all of them (grid.y); one of many has a block for every
+// tile's first adapter, and some more that look for the tiles which have others. The rows need no order and
+// the host no list of groups, so that a captured step serves whatever requests come.
 //
 // What bounds it: few rows, the latency of two launches that each wait for memory once (the factors
 // of the step's adapters are some MB); many rows, reading and writing x, base and out. h enters the
 // second product as a sum of two bfloat16 numbers (the rounded value and what the rounding left, 16
-// bits together), so that the only rounding of note is that of `out`. A lane of the second product
-// holds 16 neighbouring columns of one row: which of B's rows a tile's lane takes is free, and is
-// chosen so.
+// bits together), so that the only rounding of note is that of `out`.
 //
 // A tile's sums run in the same order however many rows the step has: every form cuts k among
 // eight waves in the same way, and a request's numbers do not depend on its company.
@@ -35,7 +34,7 @@ struct AdapterArgs {
   const int* row_adapter;   // [T]; outside [0, L): none
   const void* base;      // [T, ldb]; may be out
   void* out;             // [T, ldo]
-  float* h;              // [T, S R]
+  void* h;               // [T, S R] 32-bit numbers, or as many pairs of bfloat16 ones in two planes
   long long ldx, ldb, ldo;
   int T, K, R, S, L, N;
   int first[5];          // slice s: columns first[s] .. first[s + 1]
@@ -47,7 +46,7 @@ constexpr int kExpandWaves = 4;
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-// 16 bytes of a row, as the matrix units take them: a lane of quad q holds numbers 8 q .. 8 q + 7 of 32
+// 16 bytes of a row, as the matrix units take them: a lane of quad q (lane / 16) holds numbers 8 q .. 8 q + 7 of 32
 // (bfloat16) or 4 q .. 4 q + 3 of 16 (32-bit, whose products take 4 of k at a time: which ones is free as
 // long as both operands agree).
 template <typename T> struct Frag;
@@ -107,267 +106,431 @@ struct TileAdapters {
   }
 };
 
-// The work of a block: with `per` > 0 blocks that run on one XCD (block id mod 8) take neighbouring work, so that a
-// request's rows find its factors in that XCD's L2; -1 behind the last.
-__device__ __forceinline__ int work_of_block(int per, int total) {
-  const int b = per ? blockIdx.x % kXcds * per + blockIdx.x / kXcds : blockIdx.x;
-  return b < total ? b : -1;
+// The `u`th of all tiles' adapters but their first ones, in the order of tiles: its tile, and which of the tile's it is (-1: there
+// are fewer). By the whole block of WAVES waves: 64 tiles of 32 rows at a time, their numbers of further adapters in `counts` [64].
+template <int WAVES>
+__device__ int find_further(const AdapterArgs& a, int u, int* counts, int& tile) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, tiles = (a.T + 31) / 32;
+  for (int base = 0; base < tiles; base += 64) {
+    int of[32 / WAVES];   // a wave's pairs of tiles, a row a lane
+#pragma unroll
+    for (int i = 0; i < 32 / WAVES; ++i) {
+      const int row = (base + 2 * (w + i * WAVES)) * 32 + lane;
+      of[i] = row < a.T ? a.row_adapter[row] : -1;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 32 / WAVES; ++i) {
+      int n0 = 0, n1 = 0;
+      for (unsigned long long left = __ballot(of[i] >= 0 && of[i] < a.L); left;) {
+        const unsigned long long rows = __ballot(of[i] == __builtin_amdgcn_readlane(of[i], __ffsll(left) - 1));
+        n0 += (unsigned)rows != 0;
+        n1 += rows >> 32 != 0;
+        left &= ~rows;
+      }
+      if (lane < 2) counts[2 * (w + i * WAVES) + lane] = max((lane ? n1 : n0) - 1, 0);
+    }
+    __syncthreads();
+    const int mine = counts[lane];
+    int upto = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(upto, d, 64);
+      if (lane >= d) upto += o;
+    }
+    const unsigned long long hit = __ballot(upto > u);
+    if (hit) {
+      const int l = __ffsll(hit) - 1;
+      tile = base + l;
+      return 1 + u - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(mine, l));
+    }
+    u -= __builtin_amdgcn_readlane(upto, 63);
+  }
+  return -1;
 }
+
+// The tile and the group of columns of block `b` of the grid's x. With `near`, blocks that run on one XCD (block id mod 8) have
+// neighbouring ones, so that a request's rows find its factors in that XCD's L2. False: there is none.
+__device__ __forceinline__ bool place_of(int b, bool near, int groups, int total, int& tile, int& group) {
+  if (near) b = b % kXcds * ((total + kXcds - 1) / kXcds) + b / kXcds;
+  tile = b / groups, group = b % groups;
+  return b < total;
+}
+
+// The 16 bytes at number `k` of a row of whole such pieces, its numbers from `rank` on as 0 (whatever they are).
+template <typename T>
+__device__ __forceinline__ uint4 load_piece(const T* row, int k, int rank) {
+  if (k >= rank) return make_uint4(0, 0, 0, 0);
+  uint4 v = *(const uint4*)(row + k);
+  const int left = rank - k;   // numbers that count
+  if (left < Frag<T>::kLane) {
+    uint32_t* u = (uint32_t*)&v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int bits = (left - i * (4 / (int)sizeof(T))) * 8 * (int)sizeof(T);
+      u[i] = bits >= 32 ? u[i] : bits <= 0 ? 0u : u[i] & ((1u << bits) - 1);
+    }
+  }
+  return v;
+}
+
+// Between a wave's writes into its own shared memory and its lanes' reads of each other's: the memory itself keeps a wave's order.
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// Rows on their way to the matrix units pass through shared memory of the wave: there a lane needs 16 bytes of row `lane % 16`, and
+// such loads, whose neighbouring lanes read different rows, cost the cache four times what loads of whole lines do (2,055 rows of
+// 3,584 numbers: 42 us, of which 4 are left). 16 rows of 128 bytes, eight pieces each: piece c of row r lies at 8 r + (c ^ r / 2),
+// so that sixteen rows' pieces of one number lie in different banks. A lane loads (and puts) piece lane % 8 of rows lane / 8 and
+// lane / 8 + 8.
+__device__ __forceinline__ int place8(int row, int piece) { return row * 8 + (piece ^ (row >> 1)); }
+// ... and of 64 bytes, four pieces each.
+__device__ __forceinline__ int place4(int row, int piece) { return row * 4 + (piece ^ (row >> 2)); }
 
 // h of 16 RT rows and 16 CT columns.
 template <typename T, int RT, int CT, bool VEC>
-__global__ __launch_bounds__(kShrinkWaves * 64) void adapter_shrink_kernel(const AdapterArgs a, int groups, int per, int total) {
-  __shared__ float part[kShrinkWaves][RT * CT][64][4];
-  constexpr int kLane = Frag<T>::kLane, kStep = 4 * kLane;
-  const int b = work_of_block(per, total);
-  if (b < 0) return;
-  const int t0 = b / groups * (16 * RT), j0 = b % groups * (CT * 16);
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, quad = lane >> 4, C = a.S * a.R;
-  const T* xrow[RT];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) xrow[rt] = (const T*)a.x + (int64_t)min(t0 + rt * 16 + (lane & 15), a.T - 1) * a.ldx;
-  TileAdapters<RT> tile(a, t0);
-  for (int pass = 0; tile.left; ++pass) {
-    unsigned long long rows;
-    int rank;
-    const int g = tile.next(a, rows, rank);
-    if (pass % gridDim.y != blockIdx.y) continue;
-    bool any = false;
-    const T* arow[CT];
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      const int j = j0 + ct * 16 + (lane & 15);
-      any |= j < C && j % a.R < rank;
-      arow[ct] = (const T*)a.a + ((int64_t)g * C + min(j, C - 1)) * a.K;
+__global__ __launch_bounds__(kShrinkWaves * 64) void adapter_shrink_kernel(const AdapterArgs a, int groups, int total, int more) {
+  constexpr int F = RT + CT, kLane = Frag<T>::kLane, kStep = 8 * kLane;   // (a step: 128 bytes of each row, two products)
+  constexpr int kDepth = F <= 2 ? 4 : 2;   // steps on their way
+  constexpr int kStage = kShrinkWaves * F * 128, kPart = kShrinkWaves * RT * CT * 64;
+  __shared__ uint4 lds[kStage > kPart ? kStage : kPart];
+  // `more` > 0: tiles have a block for their first adapters only, and as many more look for the further ones; else as in the other
+  // kernel every gridDim.y'th.
+  const int first_blocks = gridDim.x - more;
+  int further = (int)blockIdx.x - first_blocks, tile_at = 0, group = 0, pass = blockIdx.y;
+  if (further < 0 && !place_of(blockIdx.x, RT > 1, groups, total, tile_at, group)) return;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, quad = lane >> 4, m = lane & 15, C = a.S * a.R;
+  const int steps = (a.K + kStep - 1) / kStep;
+  for (bool once = false;; once = true) {
+    if (once) {
+      if (more && further < 0) return;
+      pass += gridDim.y;
+      __syncthreads();   // (the memory is the next products')
     }
+    if (further >= 0) {
+      pass = find_further<kShrinkWaves>(a, further / groups, (int*)lds, tile_at);
+      if (pass < 0) return;
+      group = further % groups;
+      further += more;
+      __syncthreads();
+    }
+    const int t0 = tile_at * (16 * RT), j0 = group * (CT * 16);
+    TileAdapters<RT> tile(a, t0);
+    unsigned long long rows;
+    int rank, g = -1;
+    for (int i = 0; tile.left && i <= pass; ++i) {
+      const int next = tile.next(a, rows, rank);
+      if (i == pass) g = next;
+    }
+    if (g < 0) return;
+    bool any = false;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) any |= j0 + ct * 16 + m < C && (j0 + ct * 16 + m) % a.R < rank;
     if (!__ballot(any)) continue;
+    // row `r` of the 16 F that meet here: x's, then A's
+    auto row_of = [&](int f, int r) -> const T* {
+      if (f < RT) return (const T*)a.x + (int64_t)min(t0 + f * 16 + r, a.T - 1) * a.ldx;
+      return (const T*)a.a + ((int64_t)g * C + min(j0 + (f - RT) * 16 + r, C - 1)) * a.K;
+    };
     f32x4 acc[RT][CT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) acc[rt][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto multiply = [&](const Frag<T> (&f)[F]) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) acc[rt][ct] = Frag<T>::mma(f[rt], f[RT + ct], acc[rt][ct]);
+    };
     // wave w takes the steps w, w + 8, ..
-    int st = w;
     if constexpr (VEC) {
-      const int whole = a.K / kStep;
-#pragma unroll 4
-      for (; st < whole; st += kShrinkWaves) {
-        const int k = st * kStep + quad * kLane;
-        Frag<T> xf[RT], af[CT];
+      uint4* stage = lds + w * (F * 128);
+      const T* from[F][2];
+      uint4 next[kDepth][F][2];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) xf[rt].v = *(const decltype(xf[rt].v)*)(xrow[rt] + k);
+      for (int f = 0; f < F; ++f)
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) af[ct].v = *(const decltype(af[ct].v)*)(arow[ct] + k);
+        for (int i = 0; i < 2; ++i) from[f][i] = row_of(f, i * 8 + (lane >> 3)) + (lane & 7) * kLane;
+      auto load = [&](uint4 (&to)[F][2], int st) {
+        if ((st + 1) * kStep <= a.K) {
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
+          for (int f = 0; f < F; ++f)
 #pragma unroll
-          for (int ct = 0; ct < CT; ++ct) acc[rt][ct] = Frag<T>::mma(xf[rt], af[ct], acc[rt][ct]);
+            for (int i = 0; i < 2; ++i) to[f][i] = *(const uint4*)(from[f][i] + st * kStep);
+        } else {
+          const bool in = st * kStep + (lane & 7) * kLane < a.K;
+#pragma unroll
+          for (int f = 0; f < F; ++f)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) to[f][i] = in ? *(const uint4*)(from[f][i] + st * kStep) : make_uint4(0, 0, 0, 0);
+        }
+      };
+#pragma unroll
+      for (int d = 0; d < kDepth; ++d)
+        if (w + d * kShrinkWaves < steps) load(next[d], w + d * kShrinkWaves);
+      for (int st0 = w; st0 < steps; st0 += kDepth * kShrinkWaves) {
+#pragma unroll
+        for (int d = 0; d < kDepth; ++d) {
+          const int st = st0 + d * kShrinkWaves;
+          if (st >= steps) break;
+#pragma unroll
+          for (int f = 0; f < F; ++f)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) stage[f * 128 + place8(i * 8 + (lane >> 3), lane & 7)] = next[d][f][i];
+          if (st + kDepth * kShrinkWaves < steps) load(next[d], st + kDepth * kShrinkWaves);
+          wave_fence();
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            Frag<T> f[F];
+#pragma unroll
+            for (int i = 0; i < F; ++i) f[i].v = __builtin_bit_cast(decltype(f[i].v), stage[i * 128 + place8(m, half * 4 + quad)]);
+            multiply(f);
+          }
+          wave_fence();
+        }
       }
-    }
-    for (; st * kStep < a.K; st += kShrinkWaves) {
-      const int k = st * kStep + quad * kLane;
-      Frag<T> xf[RT];
+    } else {
+      for (int st = w; st < steps; st += kShrinkWaves) {
+#pragma unroll 1
+        for (int k = st * kStep + quad * kLane; k < (st + 1) * kStep; k += 4 * kLane) {
+          Frag<T> f[F];
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) xf[rt] = load_frag<VEC>(xrow[rt], k, a.K);
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        const Frag<T> af = load_frag<VEC>(arow[ct], k, a.K);
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) acc[rt][ct] = Frag<T>::mma(xf[rt], af, acc[rt][ct]);
-      }
-    }
-    __syncthreads();   // (the pass before has read its sums)
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) *(f32x4*)part[w][rt * CT + ct][lane] = acc[rt][ct];
-    __syncthreads();
-    for (int o = threadIdx.x; o < RT * CT * 256; o += kShrinkWaves * 64) {
-      const int f = o >> 8, l = (o >> 2) & 63, row = f / CT * 16 + (l >> 4) * 4 + (o & 3), j = j0 + f % CT * 16 + (l & 15);
-      if (!(rows >> row & 1) || j >= C || j % a.R >= rank) continue;
-      float sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < kShrinkWaves; ++i) sum += part[i][f][l][o & 3];
-      a.h[(int64_t)(t0 + row) * C + j] = sum;
-    }
-  }
-}
-
-// Numbers [at, at + kLane) of a row of h as operands: their sum is the number (one operand for 32 bits).
-template <bool VEC>
-__device__ __forceinline__ void load_h(const float* row, int at, int n, Frag<float>& f, Frag<float>&) {
-  f = load_frag<VEC>(row, at, n);
-}
-template <bool VEC>
-__device__ __forceinline__ void load_h(const float* row, int at, int n, Frag<bf16>& high, Frag<bf16>& low) {
-  float e[8];
-  const Frag<float> f0 = load_frag<VEC>(row, at, n), f1 = load_frag<VEC>(row, at + 4, n);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) e[i] = f0.v[i], e[i + 4] = f1.v[i];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    high.v[i] = (__bf16)e[i];
-    const float rest = e[i] - (float)high.v[i];
-    low.v[i] = (__bf16)(__builtin_isfinite(rest) ? rest : 0.f);   // (an infinite h leaves NaN)
-  }
-}
-
-// Sixteen neighbouring columns of a row, the ones before `n` of them; VEC: 16 bytes at a time.
-template <typename T>
-__device__ __forceinline__ void load_16(const T* p, int n, bool vec, float* f) {
-  constexpr int kEach = 16 / sizeof(T);
-  if (vec && n >= 16) {
-#pragma unroll
-    for (int i = 0; i < 16; i += kEach) {
-      const uint4 v = *(const uint4*)(p + i);
-      T e[kEach];
-      __builtin_memcpy(e, &v, 16);
-#pragma unroll
-      for (int c = 0; c < kEach; ++c) f[i + c] = to_f32(e[c]);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) f[i] = i < n ? to_f32(p[i]) : 0.f;
-  }
-}
-template <typename T>
-__device__ __forceinline__ void store_16(T* p, int n, bool vec, const float* f) {
-  constexpr int kEach = 16 / sizeof(T);
-  if (vec && n >= 16) {
-#pragma unroll
-    for (int i = 0; i < 16; i += kEach) {
-      T e[kEach];
-#pragma unroll
-      for (int c = 0; c < kEach; ++c) e[c] = from_f32<T>(f[i + c]);
-      uint4 v;
-      __builtin_memcpy(&v, e, 16);
-      *(uint4*)(p + i) = v;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (i < n) p[i] = from_f32<T>(f[i]);
-  }
-}
-
-// 64 columns a wave, 16 RT rows.
-template <typename T, int RT, bool VEC>
-__global__ __launch_bounds__(kExpandWaves * 64) void adapter_expand_kernel(const AdapterArgs a, int groups, int blocks, int per, int total,
-                                                                           bool vec_out) {
-  constexpr int kLane = Frag<T>::kLane, kStep = 4 * kLane;
-  const int b = work_of_block(per, total);
-  if (b < 0) return;
-  const int t0 = b / blocks * (16 * RT), lane = threadIdx.x & 63, quad = lane >> 4, m = lane & 15;
-  int group = b % blocks * kExpandWaves + (threadIdx.x >> 6);
-  if (group >= groups) return;
-  int s = 0;
-  for (; s < a.S - 1; ++s) {
-    const int here = (a.first[s + 1] - a.first[s] + 63) / 64;
-    if (group < here) break;
-    group -= here;
-  }
-  const int c0 = a.first[s] + group * 64, end = a.first[s + 1];
-  const int c = c0 + quad * 16, n = end - c, C = a.S * a.R;   // this lane's columns of row t0 + 16 rt + m
-  TileAdapters<RT> tile(a, t0);
-  if (a.base != a.out && blockIdx.y == 0) {
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const int t = t0 + rt * 16 + m;
-      if (t < a.T && !(tile.left >> (rt * 16 + m) & 1)) {
-        float f[16];
-        load_16((const T*)a.base + t * a.ldb + c, n, vec_out, f);
-        store_16((T*)a.out + t * a.ldo + c, n, vec_out, f);
-      }
-    }
-  }
-  for (int pass = 0; tile.left; ++pass) {
-    unsigned long long rows;
-    int rank;
-    const int g = tile.next(a, rows, rank);
-    if (pass % gridDim.y != blockIdx.y) continue;
-    const T* brow[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      brow[j] = (const T*)a.b + ((int64_t)g * a.N + min(c0 + (m >> 2) * 16 + j * 4 + (m & 3), end - 1)) * a.R;
-    f32x4 acc[RT][4];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[rt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int k0 = 0; k0 < rank; k0 += kStep) {
-      const int k = k0 + quad * kLane;
-      Frag<T> bf[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) bf[j] = load_frag<VEC>(brow[j], k, rank);
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        if (RT > 1 && !(rows >> (rt * 16) & 0xffff)) continue;
-        Frag<T> high, low;
-        load_h<VEC>(a.h + (int64_t)min(t0 + rt * 16 + m, a.T - 1) * C + s * a.R, k, rank, high, low);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          acc[rt][j] = Frag<T>::mma(bf[j], high, acc[rt][j]);
-          if constexpr (sizeof(T) == 2) acc[rt][j] = Frag<T>::mma(bf[j], low, acc[rt][j]);
+          for (int i = 0; i < F; ++i) f[i] = load_frag<false>(row_of(i, m), k, a.K);
+          multiply(f);
         }
       }
     }
-    const float scale = a.scale[g];
+    __syncthreads();
+    f32x4* part = (f32x4*)lds;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const int t = t0 + rt * 16 + m;
-      if (!(rows >> (rt * 16 + m) & 1)) continue;
-      float f[16];
-      load_16((const T*)a.base + t * a.ldb + c, n, vec_out, f);
+    for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int ct = 0; ct < CT; ++ct) part[(w * RT * CT + rt * CT + ct) * 64 + lane] = acc[rt][ct];
+    __syncthreads();
+    for (int o = threadIdx.x; o < RT * CT * 256; o += kShrinkWaves * 64) {
+      const int f = o >> 8, l = (o >> 2) & 63, row = f / CT * 16 + (l >> 4) * 4 + (o & 3), j = j0 + f % CT * 16 + (l & 15);
+      float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f[j * 4 + i] += scale * acc[rt][j][i];
+      for (int i = 0; i < kShrinkWaves; ++i) sum += ((const float*)lds)[i * (RT * CT * 256) + o];
+      if (!(rows >> row & 1) || j >= C || j % a.R >= rank) continue;
+      const int64_t at = (int64_t)(t0 + row) * C + j;
+      if constexpr (sizeof(T) == 4) {
+        ((float*)a.h)[at] = sum;
+      } else {   // two numbers whose sum it is; an infinite one is alone
+        const bf16 high = from_f32<bf16>(sum);
+        const float rest = sum - to_f32(high);
+        ((bf16*)a.h)[at] = high;
+        ((bf16*)a.h)[(int64_t)a.T * C + at] = from_f32<bf16>(__builtin_isfinite(rest) ? rest : 0.f);
       }
-      store_16((T*)a.out + t * a.ldo + c, n, vec_out, f);
     }
   }
 }
 
-// Blocks side by side for the adapters that a tile of rows may have, while the tiles are few; one goes through them all where they
-// are many.
-static int side_by_side(const AdapterArgs& a, long long blocks, int rows) {
-  const int most = std::min(std::min(rows, a.T), a.L);
-  return (int)std::max(1ll, std::min<long long>(most, 4ll * device_cu_count() / blocks));
+constexpr int kRow = 68;   // floats of a row of 64 in a wave's memory: so padded that rows' columns lie in different banks
+template <typename T> constexpr int kTerms = sizeof(T) == 2 ? 2 : 1;   // numbers whose sum is one of h
+
+// 16 RT rows from t0 on and the `set`th 64 columns, by one wave: what the tile's `pass`th adapter adds to its rows; with `copy` the
+// rows without an adapter too. False: the tile has no such adapter.
+template <typename T, int RT, bool VEC>
+__device__ __forceinline__ bool expand_tile(const AdapterArgs& a, int t0, int set, int sets, int pass, bool copy, uint4* stage, bool vec_out) {
+  constexpr int kLane = Frag<T>::kLane, kStep = 4 * kLane;   // (a step: 64 bytes of each row, one product; two for h's two numbers)
+  const int lane = threadIdx.x & 63, quad = lane >> 4, m = lane & 15, C = a.S * a.R;
+  TileAdapters<RT> tile(a, t0);
+  const unsigned long long with = tile.left;
+  unsigned long long rows = 0;
+  int rank = 0, g = -1;
+  for (int i = 0; tile.left && i <= pass; ++i) {
+    const int next = tile.next(a, rows, rank);
+    if (i == pass) g = next;
+  }
+  if (set >= sets || (g < 0 && !copy)) return g >= 0;
+  int s = 0;
+  for (; s < a.S - 1; ++s) {
+    const int here = (a.first[s + 1] - a.first[s] + 63) / 64;
+    if (set < here) break;
+    set -= here;
+  }
+  const int c0 = a.first[s] + set * 64, end = a.first[s + 1], n = min(end - c0, 64);
+  const T* base = (const T*)a.base + c0;
+  T* out = (T*)a.out + c0;
+  const T* h = (const T*)a.h + s * a.R;
+  const int64_t plane = (int64_t)a.T * C;
+
+  // Rows as they lie in memory: 16 bytes a lane, kCols of them side by side.
+  constexpr int kEach = 16 / sizeof(T), kCols = 64 / kEach, kRows = 64 / kCols;
+  const bool whole = vec_out && n == 64;
+  uint4 was[RT][16 / kRows];
+  auto load_base = [&](unsigned long long rows) {
+    if (!whole) return;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int i = 0; i < 16 / kRows; ++i) {
+        const int r = rt * 16 + i * kRows + lane / kCols;
+        if (rows >> r & 1) was[rt][i] = *(const uint4*)(base + (t0 + r) * a.ldb + lane % kCols * kEach);
+      }
+  };
+  auto store = [&](int rt, unsigned long long rows, float scale, const float* tile_) {   // tile_: rows of kRow floats, or null: 0
+    if (whole) {
+#pragma unroll
+      for (int i = 0; i < 16 / kRows; ++i) {
+        const int in = i * kRows + lane / kCols, r = rt * 16 + in;
+        if (!(rows >> r & 1)) continue;
+        T e[kEach];
+        __builtin_memcpy(e, &was[rt][i], 16);
+        if (tile_) {
+#pragma unroll
+          for (int c = 0; c < kEach; ++c) e[c] = from_f32<T>(to_f32(e[c]) + scale * tile_[in * kRow + lane % kCols * kEach + c]);
+        }
+        uint4 v;
+        __builtin_memcpy(&v, e, 16);
+        *(uint4*)(out + (t0 + r) * a.ldo + lane % kCols * kEach) = v;
+      }
+    } else {
+#pragma unroll 1
+      for (int in = 0; in < 16; ++in) {
+        const int r = rt * 16 + in;
+        if (!(rows >> r & 1) || lane >= n) continue;
+        const T v = base[(t0 + r) * a.ldb + lane];
+        out[(t0 + r) * a.ldo + lane] = tile_ ? from_f32<T>(to_f32(v) + scale * tile_[in * kRow + lane]) : v;
+      }
+    }
+  };
+
+  if (copy) {
+    unsigned long long none = ~with & ((1ull << (16 * RT)) - 1);
+    if (t0 + 16 * RT > a.T) none &= (1ull << (a.T - t0)) - 1;
+    if (none) {
+      load_base(none);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) store(rt, none, 0.f, nullptr);
+    }
+  }
+  if (g < 0) return false;
+  const float scale = a.scale[g];
+  load_base(rows);
+  auto brow = [&](int j, int r) { return (const T*)a.b + ((int64_t)g * a.N + min(c0 + j * 16 + r, end - 1)) * a.R; };
+  auto hrow = [&](int rt, int r) { return h + (int64_t)min(t0 + rt * 16 + r, a.T - 1) * C; };
+  f32x4 acc[RT][4];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[rt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int k0 = 0; k0 < rank; k0 += kStep) {
+    if constexpr (VEC) {
+      const int k = k0 + (lane & 3) * kLane, r = lane >> 2;
+      uint4 now[4 + RT * kTerms<T>];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) now[j] = load_piece(brow(j, r), k, rank);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int x = 0; x < kTerms<T>; ++x) now[4 + rt * kTerms<T> + x] = load_piece(hrow(rt, r) + x * plane, k, rank);
+#pragma unroll
+      for (int f = 0; f < 4 + RT * kTerms<T>; ++f) stage[f * 64 + place4(r, lane & 3)] = now[f];
+      wave_fence();
+      Frag<T> bf[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) bf[j].v = __builtin_bit_cast(decltype(bf[j].v), stage[j * 64 + place4(m, quad)]);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int x = 0; x < kTerms<T>; ++x) {
+          Frag<T> hf;
+          hf.v = __builtin_bit_cast(decltype(hf.v), stage[(4 + rt * kTerms<T> + x) * 64 + place4(m, quad)]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[rt][j] = Frag<T>::mma(bf[j], hf, acc[rt][j]);
+        }
+      wave_fence();
+    } else {
+      const int k = k0 + quad * kLane;
+      Frag<T> bf[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) bf[j] = load_frag<false>(brow(j, m), k, rank);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int x = 0; x < kTerms<T>; ++x) {
+          const Frag<T> hf = load_frag<false>(hrow(rt, m) + x * plane, k, rank);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[rt][j] = Frag<T>::mma(bf[j], hf, acc[rt][j]);
+        }
+    }
+  }
+  float* floats = (float*)stage;
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    if (RT > 1 && !(rows >> (rt * 16) & 0xffff)) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) *(f32x4*)(floats + m * kRow + j * 16 + quad * 4) = acc[rt][j];
+    wave_fence();
+    store(rt, rows, scale, floats);
+    wave_fence();
+  }
+  return true;
 }
+
+// Four waves take neighbouring columns.
+template <typename T, int RT, bool VEC>
+__global__ __launch_bounds__(kExpandWaves * 64) void adapter_expand_kernel(const AdapterArgs a, int sets, int groups, int total, bool vec_out) {
+  constexpr int kStage = (4 + RT * kTerms<T>) * 64, kTile = 16 * kRow / 4;
+  __shared__ uint4 lds[kExpandWaves][kStage > kTile ? kStage : kTile];
+  int tile, group;
+  if (!place_of(blockIdx.x, RT > 1, groups, total, tile, group)) return;
+  const int wave = threadIdx.x >> 6;
+  for (int pass = blockIdx.y;; pass += gridDim.y)
+    if (!expand_tile<T, RT, VEC>(a, tile * (16 * RT), group * kExpandWaves + wave, sets, pass, pass == 0 && a.base != a.out, lds[wave],
+                                 vec_out))
+      return;
+}
+
+// Adapters that a tile may have.
+static int most_adapters(const AdapterArgs& a, int rows) { return std::min(std::min(rows, a.T), a.L); }
 
 template <typename T, int RT, int CT>
 static void shrink(const AdapterArgs& a, hipStream_t stream) {
   constexpr int kLane = Frag<T>::kLane;
+  static_assert(RT == 1 || RT == 2, "find_further looks at tiles of 32 rows");
   const int groups = (a.S * a.R + CT * 16 - 1) / (CT * 16), total = (a.T + 16 * RT - 1) / (16 * RT) * groups;
-  const int per = RT > 1 ? (total + kXcds - 1) / kXcds : 0;
-  const dim3 grid(per ? per * kXcds : total, side_by_side(a, total, 16 * RT));
+  const int most = most_adapters(a, 16 * RT), cus = device_cu_count();
+  int more = 0;
+  dim3 grid;
+  if (RT == 1) {   // (four of these blocks run on a CU)
+    grid = dim3(total, std::max(1, std::min(most, 4 * cus / total)));
+  } else {         // (one does: a block that finds nothing to do would hold the place of one that has)
+    if (most > 1) more = std::min((most - 1) * total, std::max(cus - total, cus / 4));
+    grid = dim3((total + kXcds - 1) / kXcds * kXcds + more);
+  }
   const bool vec = (uintptr_t)a.x % 16 == 0 && (uintptr_t)a.a % 16 == 0 && a.K % kLane == 0 && a.ldx % kLane == 0;
-  if (vec) adapter_shrink_kernel<T, RT, CT, true><<<grid, kShrinkWaves * 64, 0, stream>>>(a, groups, per, total);
-  else adapter_shrink_kernel<T, RT, CT, false><<<grid, kShrinkWaves * 64, 0, stream>>>(a, groups, per, total);
+  if (vec) adapter_shrink_kernel<T, RT, CT, true><<<grid, kShrinkWaves * 64, 0, stream>>>(a, groups, total, more);
+  else adapter_shrink_kernel<T, RT, CT, false><<<grid, kShrinkWaves * 64, 0, stream>>>(a, groups, total, more);
 }
 
 template <typename T, int RT>
 static void expand(const AdapterArgs& a, hipStream_t stream) {
   constexpr int kLane = Frag<T>::kLane;
-  int groups = 0;
+  int sets = 0;
   bool vec_out = (uintptr_t)a.out % 16 == 0 && (uintptr_t)a.base % 16 == 0 && a.ldo * sizeof(T) % 16 == 0 && a.ldb * sizeof(T) % 16 == 0;
   for (int s = 0; s < a.S; ++s) {
-    groups += (a.first[s + 1] - a.first[s] + 63) / 64;
+    sets += (a.first[s + 1] - a.first[s] + 63) / 64;
     vec_out &= a.first[s] * sizeof(T) % 16 == 0;
   }
-  const int blocks = (groups + kExpandWaves - 1) / kExpandWaves, total = (a.T + 16 * RT - 1) / (16 * RT) * blocks;
-  const int per = RT > 1 ? (total + kXcds - 1) / kXcds : 0;
-  const dim3 grid(per ? per * kXcds : total, side_by_side(a, total, 16 * RT));
+  const int groups = (sets + kExpandWaves - 1) / kExpandWaves, total = (a.T + 16 * RT - 1) / (16 * RT) * groups;
+  const int side = std::min(most_adapters(a, 16 * RT), std::max(RT == 1 ? 1 : 4, 4 * device_cu_count() / total));
+  const dim3 grid(RT == 1 ? total : (total + kXcds - 1) / kXcds * kXcds, side);
   const bool vec = (uintptr_t)a.b % 16 == 0 && a.R % kLane == 0;
-  if (vec) adapter_expand_kernel<T, RT, true><<<grid, kExpandWaves * 64, 0, stream>>>(a, groups, blocks, per, total, vec_out);
-  else adapter_expand_kernel<T, RT, false><<<grid, kExpandWaves * 64, 0, stream>>>(a, groups, blocks, per, total, vec_out);
+  if (vec) adapter_expand_kernel<T, RT, true><<<grid, kExpandWaves * 64, 0, stream>>>(a, sets, groups, total, vec_out);
+  else adapter_expand_kernel<T, RT, false><<<grid, kExpandWaves * 64, 0, stream>>>(a, sets, groups, total, vec_out);
 }
 
 template <typename T>
 static void launch(const AdapterArgs& a, hipStream_t stream) {
   if (a.T >= 512) {
     shrink<T, 2, 4>(a, stream);
-    expand<T, 4>(a, stream);
+    expand<T, 2>(a, stream);
   } else {
     shrink<T, 1, 1>(a, stream);
     expand<T, 1>(a, stream);

@@ -69,6 +69,25 @@ def test_adapters(ops, dtype, t, k, widths, r, count, kind):
     assert torch.equal(base, out)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("t,count", [(512, 1), (600, 70), (2061, 40), (5000, 3)])
+@pytest.mark.parametrize("kind", ["one", "mixed", "portions", "last"])
+def test_adapters_of_many_rows(ops, dtype, t, count, kind):
+    """Tiles of one adapter, of as many as rows, and a step of which only the last rows have any."""
+    k, widths, r = 136, (80, 24), 8
+    rng = random.Random(t)
+    x, a, b, scale, base = tables(count, k, widths, r, dtype, t, t)
+    ranks = [rng.randint(0, r) for _ in range(count)]
+    ranks[-1] = r
+    rows = [-1] * (t - 9) + [i % count for i in range(9)] if kind == "last" else rows_of(kind, t, count, rng)
+    want, room = rc.adapters(x.cpu(), a.cpu(), b.cpu(), scale.cpu(), ranks, widths, torch.tensor(rows), base.cpu())
+    out = torch.full_like(base, NAN)
+    ops.adapter_add(x, a, b, scale, i32(ranks), widths, i32(rows), out, base=base)
+    rc.close(out, want, room)
+    ops.adapter_add(x, a, b, scale, i32(ranks), widths, i32(rows), base)
+    assert torch.equal(base, out)
+
+
 def test_adapters_rows_without_one_keep_their_bits(ops):
     x, a, b, scale, base = tables(3, 128, (64, 64), 16, torch.bfloat16, 1, 40)
     base[3, 5], base[7, 9] = NAN, INF
