@@ -8,6 +8,7 @@ loaded, `load_ops` raises.
 from __future__ import annotations
 
 import ctypes
+import struct
 import weakref
 from dataclasses import replace
 from typing import Optional
@@ -21,6 +22,7 @@ _DT = {torch.float32: 0, torch.bfloat16: 1}
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_device_now = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 class KernelError(RuntimeError):
@@ -264,33 +266,10 @@ class _GatedSumArgs(ctypes.Structure):
                 ("real", ctypes.c_int), ("dtype", ctypes.c_int), ("mult", ctypes.c_float)]
 
 
-class _AdapterArgs(ctypes.Structure):
-    _fields_ = [("x", ctypes.c_void_p), ("a", ctypes.c_void_p), ("b", ctypes.c_void_p),
-                ("scale", ctypes.c_void_p), ("ranks", ctypes.c_void_p), ("row_adapter", ctypes.c_void_p),
-                ("base", ctypes.c_void_p), ("out", ctypes.c_void_p), ("h", ctypes.c_void_p),
-                ("ldx", ctypes.c_int64), ("ldb", ctypes.c_int64), ("ldo", ctypes.c_int64),
-                ("T", ctypes.c_int), ("K", ctypes.c_int), ("R", ctypes.c_int), ("S", ctypes.c_int),
-                ("L", ctypes.c_int), ("N", ctypes.c_int), ("first", ctypes.c_int * 5), ("dtype", ctypes.c_int)]
-
-
-class _AdjustArgs(ctypes.Structure):
-    _fields_ = [("logits", ctypes.c_void_p), ("out", ctypes.c_void_p), ("repetition", ctypes.c_void_p),
-                ("presence", ctypes.c_void_p), ("frequency", ctypes.c_void_p),
-                ("hist_offsets", ctypes.c_void_p), ("hist_tokens", ctypes.c_void_p),
-                ("hist_counts", ctypes.c_void_p), ("hist_generated", ctypes.c_void_p),
-                ("bias_offsets", ctypes.c_void_p), ("bias_tokens", ctypes.c_void_p),
-                ("bias_values", ctypes.c_void_p), ("masks", ctypes.c_void_p), ("mask_rows", ctypes.c_void_p),
-                ("ld", ctypes.c_int64), ("ldo", ctypes.c_int64), ("R", ctypes.c_int), ("V", ctypes.c_int),
-                ("n_hist", ctypes.c_int), ("n_bias", ctypes.c_int), ("n_masks", ctypes.c_int),
-                ("vec", ctypes.c_int)]
-
-
-class _LogprobArgs(ctypes.Structure):
-    _fields_ = [("logits", ctypes.c_void_p), ("tokens", ctypes.c_void_p), ("logprob", ctypes.c_void_p),
-                ("before", ctypes.c_void_p), ("best", ctypes.c_void_p), ("best_logprob", ctypes.c_void_p),
-                ("sums", ctypes.c_void_p), ("counts", ctypes.c_void_p), ("keys", ctypes.c_void_p),
-                ("ld", ctypes.c_int64), ("R", ctypes.c_int), ("V", ctypes.c_int), ("top", ctypes.c_int),
-                ("vec", ctypes.c_int)]
+# Arguments of calls that a step makes many times, laid out by one call each (a ctypes structure costs the host three times as much)
+_ADAPTER_ARGS = struct.Struct("9Q3q6i5ii")    # x a b scale ranks row_adapter base out h | ldx ldb ldo | T K R S L N | first[5] | dtype
+_ADJUST_ARGS = struct.Struct("14Q2q6i")       # logits out repetition presence frequency, histories, biases, masks mask_rows | ld ldo | R V n_hist n_bias n_masks vec
+_LOGPROB_ARGS = struct.Struct("9Qq4i")        # logits tokens logprob before best best_logprob sums counts keys | ld | R V top vec
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -312,14 +291,6 @@ def _dev(t: torch.Tensor, name: str, dtype=None, dims: Optional[int] = None) -> 
         _need(t.dtype == dtype, f"{name} must be {dtype}, is {t.dtype}")
     if dims is not None:
         _need(t.dim() == dims, f"{name} must have {dims} dimensions, has {t.dim()}")
-
-
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Do two row-major [rows, columns] tensors' spans of memory meet?"""
-    def span(t):
-        return t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size()
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
 
 
 class _Together:
@@ -406,10 +377,10 @@ class HipOps:
         if self.lib.ninfer_sample_few_tokens() != self.FEW_TOKENS:
             raise KernelError(f"{self.lib_path} samples rows of up to {self.lib.ninfer_sample_few_tokens()} tokens by "
                               f"the whole GPU, these bindings say {self.FEW_TOKENS}")
-        for args, size in ((_AdapterArgs, self.lib.ninfer_adapter_args_bytes), (_AdjustArgs, self.lib.ninfer_adjust_args_bytes),
-                           (_LogprobArgs, self.lib.ninfer_logprob_args_bytes)):
-            if size() != ctypes.sizeof(args):
-                raise KernelError(f"{self.lib_path} and these bindings lay {args.__name__} out differently")
+        for args, size in ((_ADAPTER_ARGS, self.lib.ninfer_adapter_args_bytes), (_ADJUST_ARGS, self.lib.ninfer_adjust_args_bytes),
+                           (_LOGPROB_ARGS, self.lib.ninfer_logprob_args_bytes)):
+            if size() != args.size:
+                raise KernelError(f"{self.lib_path} and these bindings lay arguments out differently ({args.format})")
         self.lib.ninfer_logprob_scratch_bytes.restype = ctypes.c_longlong
         self.lib.ninfer_attention_workspace_floats.restype = ctypes.c_longlong
         self.lib.ninfer_event_create.restype = ctypes.c_void_p
@@ -417,6 +388,8 @@ class HipOps:
         self.lib.ninfer_sample_spread_bytes.restype = ctypes.c_longlong
         p, i = ctypes.c_void_p, ctypes.c_int
         self.lib.ninfer_gemm.argtypes = [p, i, p]
+        self.lib.ninfer_adapter_add.argtypes = self.lib.ninfer_adjust_logits.argtypes = [ctypes.c_char_p, p]
+        self.lib.ninfer_token_logprobs.argtypes = [ctypes.c_char_p, p, p]
         self.lib.ninfer_sample_rows.argtypes = [p, i, i, i, i, p, p, ctypes.c_longlong, i, p, p, p]
         self.lib.ninfer_latent_attention_workspace_floats.restype = ctypes.c_longlong
         self.lib.ninfer_gla_segment_floats.restype = ctypes.c_longlong
@@ -2248,50 +2221,90 @@ class HipOps:
         self._ok(self.lib.ninfer_sigmoid_attention(ctypes.byref(a), self._stream()))
 
     # ---- what single requests ask of a batch --------------------------------------------
-    def adapter_add(self, x, a, b, scale, ranks, widths, row_adapter, out, base=None):
+    # (every call's host time is that of a small step's kernels: checks are written out, the good case is one test)
+    @staticmethod
+    def _rows_of(x, dtype, who) -> int:
+        """The row stride of a row-major [rows, columns] tensor of this type on the current device; rows do not overlap."""
+        if not (x.is_cuda and x.dtype is dtype and x.dim() == 2):
+            raise KernelError(f"{who} must be rows of {dtype} on the GPU")
+        (rows, n), (ld, one) = x.shape, x.stride()
+        if rows < 2:
+            ld = max(ld, n)
+        if (one != 1 and n > 1) or ld < n:
+            raise KernelError(f"{who} must be columns of rows that do not overlap, has strides {x.stride()}")
+        return ld
+
+    @staticmethod
+    def _flat(x, dtype, n, device, name) -> int:
+        """The address of `n` numbers of this type in a row (0 for None)."""
+        if x is None:
+            return 0
+        if not (x.dtype is dtype and x.numel() == n and x.dim() == 1 and x.is_contiguous() and x.get_device() == device):
+            raise KernelError(f"{name} must be {n} numbers of {dtype} in a row, on the rows' GPU")
+        return x.data_ptr()
+
+    def _here(self, device: int) -> None:
+        """Calls go to the current stream of the current device: their tensors have to be there."""
+        if device != _device_now():
+            raise KernelError(f"tensors on cuda:{device}, but the current device is cuda:{_device_now()}")
+
+    @staticmethod
+    def _stream_of(device: int) -> int:
+        return torch.cuda.current_stream(device).cuda_stream if _raw_stream is None else _raw_stream(device)
+
+    def adapter_add(self, x, a, b, scale, ranks, widths, row_adapter, out, base=None, single_rows=0):
         """Low-rank adapters of many requests beside a projection whose output `base` [T, N] is (None: `out`, in place): for
         row t with adapter g = row_adapter[t] and every slice s of the columns (`widths`: their sizes, up to four),
         out[t, slice] = base[t, slice] + scale[g] B[g, slice] (A[g, s R : s R + ranks[g]] x[t]). x [T, K] and out [T, N]
         in bfloat16 or 32-bit, columns of wider rows if need be; a [L, len(widths) R, K] and b [L, N, R] of the same
         type, scale [L] 32-bit, ranks [L] and row_adapter [T] int32. What lies beyond an adapter's rank does not
-        count, whatever it holds. Rows whose number is outside [0, L) have no adapter: out = base."""
-        if not (x.is_cuda and x.dim() == 2 and x.dtype in _DT):
-            raise KernelError("adapter_add: x must be rows of bfloat16 or 32-bit numbers on the GPU")
-        (t, k), dt, dev = x.shape, x.dtype, x.device
-        _need(a.dim() == 3 and b.dim() == 3 and 1 <= len(widths) <= 4, "adapter_add: factors of one to four slices")
+        count, whatever it holds. Rows whose number is outside [0, L) have no adapter: out = base. `single_rows`: the first
+        so many rows are of different requests each, as a step has them; many other rows should be
+        neighbours where they share an adapter. It changes the time alone: a row's numbers are the same in any company."""
+        dt = x.dtype
+        if dt not in _DT:
+            raise KernelError(f"adapter_add: rows of {dt}")
+        in_place = base is None or base is out
+        ldx, ldo = self._rows_of(x, dt, "adapter_add: x"), self._rows_of(out, dt, "adapter_add: out")
+        ldb = ldo if in_place else self._rows_of(base, dt, "adapter_add: base")
+        dev = x.get_device()
+        (t, k), slices = x.shape, len(widths)
+        if not (a.dtype is dt and b.dtype is dt and a.dim() == 3 and b.dim() == 3 and a.is_contiguous() and b.is_contiguous()
+                and a.get_device() == dev and b.get_device() == dev and out.get_device() == dev):
+            raise KernelError(f"adapter_add: factors must be three-dimensional, contiguous and of {dt}, on the rows' GPU")
         count, n, r = b.shape
-        _need(a.shape == (count, len(widths) * r, k) and sum(widths) == n and min(widths) >= 1 and count >= 1 and r >= 1 and k >= 1,
-              f"adapter_add: factors {tuple(a.shape)} and {tuple(b.shape)} do not fit {k} columns and slices {tuple(widths)}")
-        for name, v, dtype, size in (("a", a, dt, None), ("b", b, dt, None), ("scale", scale, torch.float32, count),
-                                     ("ranks", ranks, torch.int32, count), ("row_adapter", row_adapter, torch.int32, t)):
-            _dev(v, name, dtype)
-            if not (v.device == dev and (size is None or v.shape == (size,))):
-                raise KernelError(f"adapter_add: {name} has the wrong size or device")
-        base = out if base is None else base
-        for name, v in (("out", out), ("base", base)):
-            if not (v.device == dev and v.dtype == dt and v.shape == (t, n)):
-                raise KernelError(f"adapter_add: {name} must be [{t}, {n}] of {dt}")
-        ldx, ldo, ldb = (self._columns(v, v.shape[1], "adapter_add: rows") for v in (x, out, base))
+        if not (1 <= slices <= 4 and min(widths) >= 1 and sum(widths) == n and a.shape == (count, slices * r, k) and count and r and k):
+            raise KernelError(f"adapter_add: factors {tuple(a.shape)} and {tuple(b.shape)} do not fit {k} columns and slices {tuple(widths)}")
+        if out.shape != (t, n) or not (in_place or (base.shape == (t, n) and base.get_device() == dev)):
+            raise KernelError(f"adapter_add: out and base must be [{t}, {n}], on the rows' GPU")
+        p_scale = self._flat(scale, torch.float32, count, dev, "adapter_add: scale")
+        p_ranks = self._flat(ranks, torch.int32, count, dev, "adapter_add: ranks")
+        p_rows = self._flat(row_adapter, torch.int32, t, dev, "adapter_add: row_adapter")
+        if not 0 <= single_rows <= t:
+            raise KernelError(f"adapter_add: {single_rows} single rows of {t}")
         if t == 0:
             return
-        _need(min(ldo, ldb) >= n and ldx >= 0, "adapter_add: rows that overlap")
-        _need(base is out or (base.data_ptr() == out.data_ptr() and ldb == ldo) or not _overlap(base, out),
-              "adapter_add: base and out overlap")
-        _need(not _overlap(x, out), "adapter_add: x and out overlap")
+        px, po = x.data_ptr(), out.data_ptr()
+        pb = po if in_place else base.data_ptr()
+        size = 4 if dt is torch.float32 else 2
+        end_x, end_o, end_b = (p + ((t - 1) * ld + w) * size for p, ld, w in ((px, ldx, k), (po, ldo, n), (pb, ldb, n)))
+        if px < end_o and po < end_x:
+            raise KernelError("adapter_add: x and out overlap")
+        if (pb != po or ldb != ldo) and pb < end_o and po < end_b:
+            raise KernelError("adapter_add: base and out overlap")
         self._here(dev)
-        h = torch.empty(t * a.shape[1], dtype=torch.float32, device=dev)
-        first = [0]
-        for w in widths:
-            first.append(first[-1] + w)
-        args = _AdapterArgs(x.data_ptr(), a.data_ptr(), b.data_ptr(), scale.data_ptr(), ranks.data_ptr(),
-                            row_adapter.data_ptr(), base.data_ptr(), out.data_ptr(), h.data_ptr(), ldx, ldb, ldo, t, k, r,
-                            len(widths), count, n, (ctypes.c_int * 5)(*first), _DT[dt])
-        self._ok(self.lib.ninfer_adapter_add(ctypes.byref(args), self._stream()))
-
-    def _here(self, device) -> None:
-        """Calls go to the current stream of the current device: their tensors have to be there."""
-        if device.index != torch.cuda.current_device():
-            raise KernelError(f"tensors on {device}, but the current device is cuda:{torch.cuda.current_device()}")
+        h = torch.empty(t * slices * r, dtype=torch.float32, device=x.device)
+        first = [0, n, n, n, n]
+        for i in range(1, slices):
+            first[i] = first[i - 1] + widths[i - 1]
+        lib, stream, code = self.lib, self._stream_of(dev), _DT[dt]
+        pa, p_b, ph = a.data_ptr(), b.data_ptr(), h.data_ptr()
+        # single rows are few-row tiles' work, however many rows there are behind them
+        for lo, hi in ((0, single_rows), (single_rows, t)) if 0 < single_rows < t and t >= 512 else ((0, t),):
+            args = _ADAPTER_ARGS.pack(px + lo * ldx * size, pa, p_b, p_scale, p_ranks, p_rows + 4 * lo, pb + lo * ldb * size,
+                                      po + lo * ldo * size, ph + lo * slices * r * 4, ldx, ldb, ldo, hi - lo, k, r, slices, count, n, *first, code)
+            if lib.ninfer_adapter_add(args, stream):
+                self._ok(-1)
 
     def adjust_logits(self, logits, out=None, *, repetition=None, presence=None, frequency=None, hist_offsets=None,
                       hist_tokens=None, hist_counts=None, hist_generated=None, bias_offsets=None, bias_tokens=None,
@@ -2302,46 +2315,53 @@ class HipOps:
         row's mask bars it. Per row [R]: the three penalties (32-bit, None: none) and `mask_rows` (int32, the row of
         `masks` that holds, none where it is outside them). Histories: hist_tokens, hist_counts and hist_generated
         (None: no token was generated), row r's from hist_offsets[r] to hist_offsets[r + 1]; counts of a token that stands
-        there more than once are added. Biases: bias_tokens and bias_values (32-bit) in the same way; of a token that stands
-        there more than once the last holds. masks [M, ceil(V / 32)] int32: bit t % 32 of word t // 32 set: token t is
-        allowed. Ids outside [0, V) are passed over."""
-        if not (logits.is_cuda and logits.dim() == 2 and logits.dtype == torch.float32):
-            raise KernelError("adjust_logits: logits must be rows of 32-bit floats on the GPU")
-        (r, v), dev = logits.shape, logits.device
-        out = logits if out is None else out
-        _need(out.device == dev and out.dtype == torch.float32 and out.shape == (r, v), "adjust_logits: out does not fit")
-        ld, ldo = (self._columns(x, v, "adjust_logits: rows") for x in (logits, out))
-        f32, i32 = torch.float32, torch.int32
-        n_hist, n_bias = (0 if x is None else x.shape[0] for x in (hist_tokens, bias_tokens))
-        for name, x, dtype, size in (
-                ("repetition", repetition, f32, r), ("presence", presence, f32, r), ("frequency", frequency, f32, r),
-                ("hist_offsets", hist_offsets, i32, r + 1), ("hist_tokens", hist_tokens, i32, n_hist),
-                ("hist_counts", hist_counts, i32, n_hist), ("hist_generated", hist_generated, i32, n_hist),
-                ("bias_offsets", bias_offsets, i32, r + 1), ("bias_tokens", bias_tokens, i32, n_bias),
-                ("bias_values", bias_values, f32, n_bias), ("mask_rows", mask_rows, i32, r)):
-            if x is not None:
-                _dev(x, name, dtype, 1)
-                if not (x.shape[0] == size and x.device == dev):
-                    raise KernelError(f"adjust_logits: {name} has the wrong size or device")
-        _need((hist_offsets is None) == (hist_tokens is None) == (hist_counts is None)
-              and (hist_generated is None or hist_tokens is not None), "adjust_logits: a history is offsets, tokens and counts")
-        _need((bias_offsets is None) == (bias_tokens is None) == (bias_values is None),
-              "adjust_logits: biases are offsets, tokens and values")
-        _need((masks is None) == (mask_rows is None), "adjust_logits: masks and the rows' choice of them go together")
-        if masks is not None:
-            _dev(masks, "masks", i32, 2)
-            _need(masks.shape[1] == (v + 31) // 32 and masks.device == dev, "adjust_logits: masks have a bit for every token")
+        there more than once are added (sums below 2^31). Biases: bias_tokens and bias_values (32-bit) in the same way; of a
+        token that stands there more than once the last holds. masks [M, ceil(V / 32)] int32: bit t % 32 of word t // 32 set:
+        token t is allowed. Ids outside [0, V) are passed over."""
+        f32, i32, flat = torch.float32, torch.int32, self._flat
+        ld = self._rows_of(logits, f32, "adjust_logits: logits")
+        if out is None:
+            out = logits
+        ldo = ld if out is logits else self._rows_of(out, f32, "adjust_logits: out")
+        (r, v), dev = logits.shape, logits.get_device()
+        if out.shape != (r, v) or out.get_device() != dev:
+            raise KernelError(f"adjust_logits: out must be [{r}, {v}], on the rows' GPU")
+        p_rep = flat(repetition, f32, r, dev, "adjust_logits: repetition")
+        p_pres = flat(presence, f32, r, dev, "adjust_logits: presence")
+        p_freq = flat(frequency, f32, r, dev, "adjust_logits: frequency")
+        n_hist = n_bias = n_masks = ho = ht = hc = hg = bo = bt = bv = pm = mr = 0
+        if hist_offsets is not None or hist_tokens is not None or hist_counts is not None or hist_generated is not None:
+            if hist_offsets is None or hist_tokens is None or hist_counts is None:
+                raise KernelError("adjust_logits: a history is offsets, tokens and counts")
+            n_hist = hist_tokens.numel()
+            ho = flat(hist_offsets, i32, r + 1, dev, "adjust_logits: hist_offsets")
+            ht = flat(hist_tokens, i32, n_hist, dev, "adjust_logits: hist_tokens")
+            hc = flat(hist_counts, i32, n_hist, dev, "adjust_logits: hist_counts")
+            hg = flat(hist_generated, i32, n_hist, dev, "adjust_logits: hist_generated")
+        if bias_offsets is not None or bias_tokens is not None or bias_values is not None:
+            if bias_offsets is None or bias_tokens is None or bias_values is None:
+                raise KernelError("adjust_logits: biases are offsets, tokens and values")
+            n_bias = bias_tokens.numel()
+            bo = flat(bias_offsets, i32, r + 1, dev, "adjust_logits: bias_offsets")
+            bt = flat(bias_tokens, i32, n_bias, dev, "adjust_logits: bias_tokens")
+            bv = flat(bias_values, f32, n_bias, dev, "adjust_logits: bias_values")
+        if masks is not None or mask_rows is not None:
+            if masks is None or mask_rows is None:
+                raise KernelError("adjust_logits: masks and the rows' choice of them go together")
+            if not (masks.dtype is i32 and masks.dim() == 2 and masks.shape[1] == (v + 31) // 32 and masks.is_contiguous()
+                    and masks.get_device() == dev):
+                raise KernelError(f"adjust_logits: masks must be contiguous rows of {(v + 31) // 32} words (int32), on the rows' GPU")
+            n_masks, pm = masks.shape[0], masks.data_ptr()
+            mr = flat(mask_rows, i32, r, dev, "adjust_logits: mask_rows")
         if r == 0 or v == 0:
             return
-        _need(min(ld, ldo) >= v, "adjust_logits: rows that overlap")
-        _need(out is logits or (out.data_ptr() == logits.data_ptr() and ld == ldo) or not _overlap(logits, out),
-              "adjust_logits: logits and out overlap")
+        p, po = logits.data_ptr(), out.data_ptr()
+        if (p != po or ld != ldo) and p < po + ((r - 1) * ldo + v) * 4 and po < p + ((r - 1) * ld + v) * 4:
+            raise KernelError("adjust_logits: logits and out overlap")
         self._here(dev)
-        args = _AdjustArgs(logits.data_ptr(), out.data_ptr(), _ptr(repetition), _ptr(presence), _ptr(frequency),
-                           _ptr(hist_offsets), _ptr(hist_tokens), _ptr(hist_counts), _ptr(hist_generated),
-                           _ptr(bias_offsets), _ptr(bias_tokens), _ptr(bias_values), _ptr(masks), _ptr(mask_rows), ld, ldo,
-                           r, v, n_hist, n_bias, 0 if masks is None else masks.shape[0], 0)
-        self._ok(self.lib.ninfer_adjust_logits(ctypes.byref(args), self._stream()))
+        args = _ADJUST_ARGS.pack(p, po, p_rep, p_pres, p_freq, ho, ht, hc, hg, bo, bt, bv, pm, mr, ld, ldo, r, v, n_hist, n_bias, n_masks, 0)
+        if self.lib.ninfer_adjust_logits(args, self._stream_of(dev)):
+            self._ok(-1)
 
     LISTED_TOKENS = 64   # most tokens of a row whose log-probabilities `token_logprobs` lists
 
@@ -2351,27 +2371,24 @@ class HipOps:
         by logit, of equal ones the lower id first. Without `tokens` (int32) the first two are None; for a token outside
         [0, V) they are NaN and -1. A row of nothing but -inf has log-probabilities of -inf; a NaN makes all of its row's NaN
         and stands behind every other token."""
-        if not (logits.is_cuda and logits.dim() == 2 and logits.dtype == torch.float32):
-            raise KernelError("token_logprobs: logits must be rows of 32-bit floats on the GPU")
-        (r, v), dev = logits.shape, logits.device
-        ld = self._columns(logits, v, "token_logprobs: rows")
-        if not (0 <= top <= min(self.LISTED_TOKENS, v)):
+        f32, i32 = torch.float32, torch.int32
+        ld = self._rows_of(logits, f32, "token_logprobs: logits")
+        (r, v), dev, device = logits.shape, logits.get_device(), logits.device
+        if not 0 <= top <= min(self.LISTED_TOKENS, v):
             raise KernelError(f"token_logprobs: top {top} is outside [0, {min(self.LISTED_TOKENS, v)}]")
+        pt = self._flat(tokens, i32, r, dev, "token_logprobs: tokens")
+        self._here(dev)
         logprob = before = None
+        pl = pbf = 0
         if tokens is not None:
-            _dev(tokens, "tokens", torch.int32, 1)
-            _need(tokens.shape[0] == r and tokens.device == dev, "token_logprobs: one token a row")
-            logprob = torch.empty(r, dtype=torch.float32, device=dev)
-            before = torch.empty(r, dtype=torch.int32, device=dev)
-        best = torch.empty((r, top), dtype=torch.int32, device=dev)
-        best_logprob = torch.empty((r, top), dtype=torch.float32, device=dev)
+            logprob, before = torch.empty(r, dtype=f32, device=device), torch.empty(r, dtype=i32, device=device)
+            pl, pbf = logprob.data_ptr(), before.data_ptr()
+        best, best_logprob = torch.empty((r, top), dtype=i32, device=device), torch.empty((r, top), dtype=f32, device=device)
         if r and v and (top or tokens is not None):
-            _need(ld >= v, "token_logprobs: rows that overlap")
-            self._here(dev)
-            scratch = torch.empty(self.lib.ninfer_logprob_scratch_bytes(r, v, top), dtype=torch.uint8, device=dev)
-            args = _LogprobArgs(logits.data_ptr(), _ptr(tokens), _ptr(logprob), _ptr(before), best.data_ptr(),
-                                best_logprob.data_ptr(), None, None, None, ld, r, v, top, 0)
-            self._ok(self.lib.ninfer_token_logprobs(ctypes.byref(args), ctypes.c_void_p(scratch.data_ptr()), self._stream()))
+            scratch = torch.empty(self.lib.ninfer_logprob_scratch_bytes(r, v, top), dtype=torch.uint8, device=device)
+            args = _LOGPROB_ARGS.pack(logits.data_ptr(), pt, pl, pbf, best.data_ptr(), best_logprob.data_ptr(), 0, 0, 0, ld, r, v, top, 0)
+            if self.lib.ninfer_token_logprobs(args, scratch.data_ptr(), self._stream_of(dev)):
+                self._ok(-1)
         return logprob, before, best, best_logprob
 
     # ---- sampling -------------------------------------------------------------------

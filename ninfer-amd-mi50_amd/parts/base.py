@@ -251,7 +251,7 @@ class AdapterSpot:
         """What the adapters of the step's rows add to the product's rows `out` of x, in place."""
         if ctx.row_adapter is not None and self.tables is not None:
             t = self.tables
-            ctx.ops.adapter_add(x, t.a, t.b, t.scale, t.ranks, t.widths, ctx.row_adapter, out)
+            ctx.ops.adapter_add(x, t.a, t.b, t.scale, t.ranks, t.widths, ctx.row_adapter, out, single_rows=ctx.single_rows)
 
 
 @dataclass

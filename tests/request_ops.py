@@ -12,7 +12,7 @@ from plain_ops import PlainOps
 class PlainRequestOps(PlainOps):
     LISTED_TOKENS = 64
 
-    def adapter_add(self, x, a, b, scale, ranks, widths, row_adapter, out, base=None):
+    def adapter_add(self, x, a, b, scale, ranks, widths, row_adapter, out, base=None, single_rows=0):
         want, _ = rc.adapters(x, a, b, scale, ranks.tolist(), widths, row_adapter, out if base is None else base)
         out.copy_(want)
 

@@ -84,6 +84,9 @@ def test_adapters_of_many_rows(ops, dtype, t, count, kind):
     out = torch.full_like(base, NAN)
     ops.adapter_add(x, a, b, scale, i32(ranks), widths, i32(rows), out, base=base)
     rc.close(out, want, room)
+    split = torch.full_like(base, NAN)
+    ops.adapter_add(x, a, b, scale, i32(ranks), widths, i32(rows), split, base=base, single_rows=37)   # the same bits
+    assert torch.equal(split, out)
     ops.adapter_add(x, a, b, scale, i32(ranks), widths, i32(rows), base)
     assert torch.equal(base, out)
 
@@ -193,6 +196,9 @@ def test_adapters_refusals(ops):
         ops.adapter_add(x, a, b, scale, ranks, (32, 32), rows, wide[1:], base=wide[:4])
     with pytest.raises(KernelError, match="overlap"):
         ops.adapter_add(x, a, b, scale, ranks, (32, 32), rows, x)
+    for single in (-1, 5):
+        with pytest.raises(KernelError, match="single rows"):
+            ops.adapter_add(x, a, b, scale, ranks, (32, 32), rows, base, single_rows=single)
     assert torch.equal(base, before)
     ops.adapter_add(x[:0], a, b, scale, ranks, (32, 32), rows[:0], base[:0])   # no rows: nothing to do
 

@@ -407,38 +407,41 @@ def refuses(lib, call, match):
 
 def test_the_library_refuses(lib):
     """Calls that end before anything is launched (no GPU here): sizes, strides, arrays that are missing."""
-    from ninfer_amd.kernels.ops import _AdapterArgs, _AdjustArgs, _LogprobArgs
+    from ninfer_amd.kernels.ops import _ADAPTER_ARGS, _ADJUST_ARGS, _LOGPROB_ARGS
     p = 1 << 20
+    fields = {_ADAPTER_ARGS: "x a b scale ranks row_adapter base out h ldx ldb ldo T K R S L N first dtype",
+              _ADJUST_ARGS: "logits out repetition presence frequency hist_offsets hist_tokens hist_counts hist_generated bias_offsets bias_tokens "
+                            "bias_values masks mask_rows ld ldo R V n_hist n_bias n_masks vec",
+              _LOGPROB_ARGS: "logits tokens logprob before best best_logprob sums counts keys ld R V top vec"}
 
-    def fill(cls, **kw):
-        a = cls()
-        for k, v in kw.items():
-            setattr(a, k, v)
-        return a
+    def fill(args, **kw):
+        values = [kw.pop(name, 0) for name in fields[args].split()]
+        assert not kw
+        return args.pack(*[x for v in values for x in (v if isinstance(v, list) else [v or 0])])
 
-    first = (ctypes.c_int * 5)(0, 64, 96)
+    first = [0, 64, 96, 0, 0]
     fine = dict(x=p, a=p, b=p, scale=p, ranks=p, row_adapter=p, base=p, out=p, h=p, ldx=64, ldb=96, ldo=96, T=4, K=64, R=8, S=2, L=2, N=96,
                 first=first, dtype=1)
     for change, match in ((dict(T=0), "positive"), (dict(K=0), "positive"), (dict(R=-1), "positive"), (dict(L=0), "positive"), (dict(S=0), "slices"),
-                          (dict(S=5), "slices"), (dict(N=95), "slices"), (dict(first=(ctypes.c_int * 5)(0, 96, 96)), "no columns"),
+                          (dict(S=5), "slices"), (dict(N=95), "slices"), (dict(first=[0, 96, 96, 0, 0]), "no columns"),
                           (dict(x=None), "null"), (dict(h=None), "null"), (dict(row_adapter=None), "null"), (dict(ldx=63), "stride"),
                           (dict(ldo=95), "stride"), (dict(ldb=200), "two row strides"), (dict(dtype=2), "dtype"),
                           (dict(T=2 ** 31 - 1), "too many")):
-        refuses(lib, lambda: lib.ninfer_adapter_add(ctypes.byref(fill(_AdapterArgs, **dict(fine, **change))), None), match)
+        refuses(lib, lambda: lib.ninfer_adapter_add(fill(_ADAPTER_ARGS, **dict(fine, **change)), None), match)
     refuses(lib, lambda: lib.ninfer_adapter_add(None, None), "no arguments")
     fine = dict(logits=p, out=p, ld=100, ldo=100, R=2, V=100)
     for change, match in ((dict(R=0), "positive"), (dict(V=-1), "positive"), (dict(logits=None), "null"), (dict(ld=99), "stride"), (dict(ldo=104), "two row strides"),
                           (dict(n_hist=-1), "negative"), (dict(hist_offsets=p, n_hist=3), "history"), (dict(bias_offsets=p, n_bias=3), "biases"),
                           (dict(mask_rows=p, n_masks=1), "masks"), (dict(R=2 ** 31 - 1, V=100000, ld=100000, ldo=100000), "too many")):
-        refuses(lib, lambda: lib.ninfer_adjust_logits(ctypes.byref(fill(_AdjustArgs, **dict(fine, **change))), None), match)
+        refuses(lib, lambda: lib.ninfer_adjust_logits(fill(_ADJUST_ARGS, **dict(fine, **change)), None), match)
     refuses(lib, lambda: lib.ninfer_adjust_logits(None, None), "no arguments")
     fine = dict(logits=p, tokens=p, logprob=p, before=p, best=p, best_logprob=p, ld=100, R=2, V=100, top=3)
     at = ctypes.c_void_p(p)
     for change, match in ((dict(R=0), "positive"), (dict(V=0), "positive"), (dict(logits=None), "null"), (dict(ld=99), "stride"), (dict(top=65), "outside"),
                           (dict(top=-1), "outside"), (dict(V=2, top=3), "outside"), (dict(logprob=None), "place"), (dict(best=None), "place"),
                           (dict(tokens=None, top=0), "nothing"), (dict(R=2 ** 31 - 1, V=100000, ld=100000), "too many")):
-        refuses(lib, lambda: lib.ninfer_token_logprobs(ctypes.byref(fill(_LogprobArgs, **dict(fine, **change))), at, None), match)
-    refuses(lib, lambda: lib.ninfer_token_logprobs(ctypes.byref(fill(_LogprobArgs, **fine)), ctypes.c_void_p(p + 8), None), "aligned")
+        refuses(lib, lambda: lib.ninfer_token_logprobs(fill(_LOGPROB_ARGS, **dict(fine, **change)), at, None), match)
+    refuses(lib, lambda: lib.ninfer_token_logprobs(fill(_LOGPROB_ARGS, **fine), ctypes.c_void_p(p + 8), None), "aligned")
     refuses(lib, lambda: lib.ninfer_token_logprobs(None, at, None), "no arguments")
     assert lib.ninfer_logprob_scratch_bytes(2, 4097, 0) == 4 * 8 + 16
     assert lib.ninfer_logprob_scratch_bytes(2, 4097, 1) == 4 * 8 + 16 + 4 * 256 * 4
