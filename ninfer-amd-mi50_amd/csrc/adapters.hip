@@ -191,7 +191,7 @@ __device__ __forceinline__ int place4(int row, int piece) { return row * 4 + (pi
 
 // h of 16 RT rows and 16 CT columns.
 template <typename T, int RT, int CT, bool VEC>
-__global__ __launch_bounds__(kShrinkWaves * 64) void adapter_shrink_kernel(const AdapterArgs a, int groups, int total, int more) {
+__global__ __launch_bounds__(kShrinkWaves * 64, RT == 1 ? 4 : 2) void adapter_shrink_kernel(const AdapterArgs a, int groups, int total, int more) {
   constexpr int F = RT + CT, kLane = Frag<T>::kLane, kStep = 8 * kLane;   // (a step: 128 bytes of each row, two products)
   constexpr int kDepth = F <= 2 ? 4 : 2;   // steps on their way
   constexpr int kStage = kShrinkWaves * F * 128, kPart = kShrinkWaves * RT * CT * 64;
@@ -338,15 +338,7 @@ template <typename T, int RT, bool VEC>
 __device__ __forceinline__ bool expand_tile(const AdapterArgs& a, int t0, int set, int sets, int pass, bool copy, uint4* stage, bool vec_out) {
   constexpr int kLane = Frag<T>::kLane, kStep = 4 * kLane;   // (a step: 64 bytes of each row, one product; two for h's two numbers)
   const int lane = threadIdx.x & 63, quad = lane >> 4, m = lane & 15, C = a.S * a.R;
-  TileAdapters<RT> tile(a, t0);
-  const unsigned long long with = tile.left;
-  unsigned long long rows = 0;
-  int rank = 0, g = -1;
-  for (int i = 0; tile.left && i <= pass; ++i) {
-    const int next = tile.next(a, rows, rank);
-    if (i == pass) g = next;
-  }
-  if (set >= sets || (g < 0 && !copy)) return g >= 0;
+  if (set >= sets) return false;
   int s = 0;
   for (; s < a.S - 1; ++s) {
     const int here = (a.first[s + 1] - a.first[s] + 63) / 64;
@@ -400,18 +392,23 @@ __device__ __forceinline__ bool expand_tile(const AdapterArgs& a, int t0, int se
     }
   };
 
-  if (copy) {
-    unsigned long long none = ~with & ((1ull << (16 * RT)) - 1);
-    if (t0 + 16 * RT > a.T) none &= (1ull << (a.T - t0)) - 1;
-    if (none) {
-      load_base(none);
+  // (on their way before the rows' adapters are known: nearly all of them are needed)
+  const unsigned long long here = (1ull << min(16 * RT, a.T - t0)) - 1;
+  if (pass == 0) load_base(here);
+  TileAdapters<RT> tile(a, t0);
+  if (copy && (here & ~tile.left)) {
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) store(rt, none, 0.f, nullptr);
-    }
+    for (int rt = 0; rt < RT; ++rt) store(rt, here & ~tile.left, 0.f, nullptr);
+  }
+  unsigned long long rows = 0;
+  int rank = 0, g = -1;
+  for (int i = 0; tile.left && i <= pass; ++i) {
+    const int next = tile.next(a, rows, rank);
+    if (i == pass) g = next;
   }
   if (g < 0) return false;
   const float scale = a.scale[g];
-  load_base(rows);
+  if (pass) load_base(rows);
   auto brow = [&](int j, int r) { return (const T*)a.b + ((int64_t)g * a.N + min(c0 + j * 16 + r, end - 1)) * a.R; };
   auto hrow = [&](int rt, int r) { return h + (int64_t)min(t0 + rt * 16 + r, a.T - 1) * C; };
   f32x4 acc[RT][4];

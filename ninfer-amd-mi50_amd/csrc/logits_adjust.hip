@@ -47,22 +47,26 @@ __device__ __forceinline__ float penalised(float l, float p, unsigned count) {
 struct AdjustLds {
   // By token of the part: first what the list's entries say of it (0: nothing), then kListed and a 32-bit float.
   unsigned long long of[kAdjustPart];
-  // The tokens of the part that stand in the list, as many as leave room for four blocks' memory on a CU; any further ones are
-  // found in `of`.
-  unsigned short listed[kAdjustPart - 4];
-  int n_listed;
+  // Entries of the list whose token lies in the part, as many as there is room for (the others are read where they are found):
+  // kEntry * the entry, from the list's first on, and the token. Then the tokens of these entries. Their memory leaves room for four
+  // blocks on a CU.
+  unsigned entry[kAdjustPart / 2 - 2];
+  int n_entries, n_listed;
 };
 static_assert(sizeof(AdjustLds) <= 40960, "four blocks to a CU");
 constexpr unsigned long long kListed = 1ull << 63;
+constexpr unsigned kEntry = kAdjustPart, kMostEntries = kAdjustPart / 2 - 2;
+constexpr int kEntriesEach = (kMostEntries + kAdjustThreads - 1) / kAdjustThreads;
 
 // One list of the row, entries [first, end): `note(entry, token)` puts an entry of the part into l.of and says whether it is
 // its token's first; `value(token, what l.of has)` makes a float of that; `put(logit, float)` goes over the listed tokens' logits.
-// The values are made by as many threads as tokens are listed: as a branch over the logits that a thread holds, nearly every wave would
-// run a power and a quotient in 64 bits for each of them (64 rows of 151,936 tokens and 2,500 entries 37 us so).
+// What an entry says is read, and the values are made, by as many threads as there are entries and tokens of the part: in the
+// loop over the list, or over the logits that a thread holds, nearly every wave would wait for those loads, and run a power and a
+// quotient in 64 bits, in every turn (256 rows of 151,936 tokens with 6,000 entries each, us: 181 so, 141 with the values alone
+// made so).
 template <typename Note, typename Value, typename Put>
 __device__ __forceinline__ bool apply_list(AdjustLds& l, const int* tokens, int first, int end, int t0, int n,
                                            float (&v)[kAdjustQuads][4], Note note, Value value, Put put) {
-  constexpr int kMost = kAdjustPart - 4;
   const int tid = threadIdx.x;
   int t[kAdjustLists];
   auto load = [&](int e0) {
@@ -73,7 +77,7 @@ __device__ __forceinline__ bool apply_list(AdjustLds& l, const int* tokens, int 
   __syncthreads();   // (the list before has been put)
 #pragma unroll
   for (int i = 0; i < kAdjustPart / kAdjustThreads; ++i) l.of[i * kAdjustThreads + tid] = 0;
-  if (tid == 0) l.n_listed = 0;
+  if (tid == 0) l.n_entries = l.n_listed = 0;
   __syncthreads();
   for (int e0 = first + tid; e0 < end; e0 += kAdjustLists * kAdjustThreads) {
     if (e0 != first + tid) load(e0);
@@ -81,25 +85,38 @@ __device__ __forceinline__ bool apply_list(AdjustLds& l, const int* tokens, int 
     for (int u = 0; u < kAdjustLists; ++u) {
       const int e = e0 + u * kAdjustThreads;
       const unsigned at = (unsigned)t[u] - (unsigned)t0;   // (ids outside the vocabulary fall outside every part)
-      if (e < end && at < (unsigned)n && note(e, (int)at)) {
-        const int i = atomicAdd(&l.n_listed, 1);
-        if (i < kMost) l.listed[i] = (unsigned short)at;
+      if (e < end && at < (unsigned)n) {
+        const unsigned i = (unsigned)(e - first) < 0xffffffffu / kEntry ? atomicAdd(&l.n_entries, 1) : kMostEntries;
+        if (i < kMostEntries) l.entry[i] = (unsigned)(e - first) * kEntry + at;
+        else note(e, (int)at);   // (its token, if this is its first entry, is found in `of`)
       }
     }
   }
   __syncthreads();
+  const int entries = min(l.n_entries, (int)kMostEntries);
+  const bool all = l.n_entries <= (int)kMostEntries && (unsigned)(end - first) < 0xffffffffu / kEntry;
+  unsigned mine[kEntriesEach];
+#pragma unroll
+  for (int u = 0; u < kEntriesEach; ++u) mine[u] = tid + u * kAdjustThreads < entries ? l.entry[tid + u * kAdjustThreads] : 0;
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kEntriesEach; ++u) {
+    const int at = mine[u] % kEntry;
+    if (tid + u * kAdjustThreads < entries && note(first + (int)(mine[u] / kEntry), at)) l.entry[atomicAdd(&l.n_listed, 1)] = at;
+  }
+  __syncthreads();
   const int listed = l.n_listed;
-  for (int i = tid; i < min(listed, kMost); i += kAdjustThreads) {
-    const int at = l.listed[i];
+  for (int i = tid; i < listed; i += kAdjustThreads) {
+    const int at = l.entry[i];
     l.of[at] = kListed | __float_as_uint(value(at, l.of[at]));
   }
   __syncthreads();
-  if (listed > kMost) {
+  if (!all) {   // (tokens of other entries)
     for (int at = tid; at < kAdjustPart; at += kAdjustThreads)
       if (l.of[at] && !(l.of[at] & kListed)) l.of[at] = kListed | __float_as_uint(value(at, l.of[at]));
     __syncthreads();
   }
-  if (listed) {
+  if (listed || !all) {
 #pragma unroll
     for (int u = 0; u < kAdjustQuads; ++u) {
 #pragma unroll
@@ -109,7 +126,7 @@ __device__ __forceinline__ bool apply_list(AdjustLds& l, const int* tokens, int 
       }
     }
   }
-  return listed > 0;
+  return listed > 0 || !all;
 }
 
 __global__ __launch_bounds__(kAdjustThreads) void adjust_logits_kernel(const AdjustArgs a, int parts) {
