@@ -39,6 +39,7 @@ struct AdapterArgs {
   int T, K, R, S, L, N;
   int first[5];          // slice s: columns first[s] .. first[s + 1]
   int dtype;
+  int single;            // the rows are of different requests each
 };
 
 constexpr int kShrinkWaves = 8;
@@ -470,37 +471,45 @@ __device__ __forceinline__ bool expand_tile(const AdapterArgs& a, int t0, int se
   return true;
 }
 
-// Four waves take neighbouring columns.
+// Four waves take neighbouring columns. `more`: as in the other kernel.
 template <typename T, int RT, bool VEC>
-__global__ __launch_bounds__(kExpandWaves * 64) void adapter_expand_kernel(const AdapterArgs a, int sets, int groups, int total, bool vec_out) {
+__global__ __launch_bounds__(kExpandWaves * 64) void adapter_expand_kernel(const AdapterArgs a, int sets, int groups, int total, int more,
+                                                                           bool vec_out) {
   constexpr int kStage = (4 + RT * kTerms<T>) * 64, kTile = 16 * kRow / 4;
   __shared__ uint4 lds[kExpandWaves][kStage > kTile ? kStage : kTile];
-  int tile, group;
-  if (!place_of(blockIdx.x, RT > 1, groups, total, tile, group)) return;
+  __shared__ int counts[64];
+  int further = (int)blockIdx.x < more ? (int)blockIdx.x : -1, tile = 0, group = 0, pass = blockIdx.y;
+  if (further < 0 && !place_of(blockIdx.x - more, RT > 1, groups, total, tile, group)) return;
   const int wave = threadIdx.x >> 6;
-  for (int pass = blockIdx.y;; pass += gridDim.y)
-    if (!expand_tile<T, RT, VEC>(a, tile * (16 * RT), group * kExpandWaves + wave, sets, pass, pass == 0 && a.base != a.out, lds[wave],
-                                 vec_out))
-      return;
+  for (;; pass += gridDim.y) {
+    if (further >= 0) {
+      pass = find_further<kExpandWaves>(a, further / groups, counts, tile);
+      if (pass < 0) return;
+      group = further % groups;
+      further += more;
+    }
+    const bool had = expand_tile<T, RT, VEC>(a, tile * (16 * RT), group * kExpandWaves + wave, sets, pass, pass == 0 && a.base != a.out,
+                                             lds[wave], vec_out);
+    if (further < 0 && (more || !had)) return;
+  }
 }
 
-// Adapters that a tile may have.
-static int most_adapters(const AdapterArgs& a, int rows) { return std::min(std::min(rows, a.T), a.L); }
+// The grid of a kernel for which the tiles' first adapters are `total` blocks' work.
+template <int RT>
+static dim3 grid_of(const AdapterArgs& a, int total, int* more) {
+  static_assert(RT == 1 || RT == 2, "find_further looks at tiles of 32 rows");
+  const int most = std::min(std::min(16 * RT, a.T), a.L), cus = device_cu_count();   // adapters that a tile may have
+  if (RT == 1) return dim3(total, std::max(1, std::min(most, 4 * cus / total)));
+  if (most > 1) *more = (int)std::min<long long>((most - 1ll) * total, std::max(cus - total, cus));
+  return dim3((total + kXcds - 1) / kXcds * kXcds + *more);
+}
 
 template <typename T, int RT, int CT>
 static void shrink(const AdapterArgs& a, hipStream_t stream) {
   constexpr int kLane = Frag<T>::kLane;
-  static_assert(RT == 1 || RT == 2, "find_further looks at tiles of 32 rows");
   const int groups = (a.S * a.R + CT * 16 - 1) / (CT * 16), total = (a.T + 16 * RT - 1) / (16 * RT) * groups;
-  const int most = most_adapters(a, 16 * RT), cus = device_cu_count();
   int more = 0;
-  dim3 grid;
-  if (RT == 1) {   // (four of these blocks run on a CU)
-    grid = dim3(total, std::max(1, std::min(most, 4 * cus / total)));
-  } else {         // (one does: a block that finds nothing to do would hold the place of one that has)
-    if (most > 1) more = std::min((most - 1) * total, std::max(cus - total, cus / 4));
-    grid = dim3((total + kXcds - 1) / kXcds * kXcds + more);
-  }
+  const dim3 grid = grid_of<RT>(a, total, &more);
   const bool vec = (uintptr_t)a.x % 16 == 0 && (uintptr_t)a.a % 16 == 0 && a.K % kLane == 0 && a.ldx % kLane == 0;
   if (vec) adapter_shrink_kernel<T, RT, CT, true><<<grid, kShrinkWaves * 64, 0, stream>>>(a, groups, total, more);
   else adapter_shrink_kernel<T, RT, CT, false><<<grid, kShrinkWaves * 64, 0, stream>>>(a, groups, total, more);
@@ -516,16 +525,19 @@ static void expand(const AdapterArgs& a, hipStream_t stream) {
     vec_out &= a.first[s] * sizeof(T) % 16 == 0;
   }
   const int groups = (sets + kExpandWaves - 1) / kExpandWaves, total = (a.T + 16 * RT - 1) / (16 * RT) * groups;
-  const int side = std::min(most_adapters(a, 16 * RT), std::max(RT == 1 ? 1 : 4, 4 * device_cu_count() / total));
-  const dim3 grid(RT == 1 ? total : (total + kXcds - 1) / kXcds * kXcds, side);
+  int more = 0;
+  const dim3 grid = grid_of<RT>(a, total, &more);
   const bool vec = (uintptr_t)a.b % 16 == 0 && a.R % kLane == 0;
-  if (vec) adapter_expand_kernel<T, RT, true><<<grid, kExpandWaves * 64, 0, stream>>>(a, sets, groups, total, vec_out);
-  else adapter_expand_kernel<T, RT, false><<<grid, kExpandWaves * 64, 0, stream>>>(a, sets, groups, total, vec_out);
+  if (vec) adapter_expand_kernel<T, RT, true><<<grid, kExpandWaves * 64, 0, stream>>>(a, sets, groups, total, more, vec_out);
+  else adapter_expand_kernel<T, RT, false><<<grid, kExpandWaves * 64, 0, stream>>>(a, sets, groups, total, more, vec_out);
 }
+
+// Rows from which tiles of 32 are the faster ones, unless every row has an adapter of its own.
+constexpr int kManyRows = 512;
 
 template <typename T>
 static void launch(const AdapterArgs& a, hipStream_t stream) {
-  if (a.T >= 512) {
+  if (a.T >= kManyRows && !a.single) {
     shrink<T, 2, 4>(a, stream);
     expand<T, 2>(a, stream);
   } else {

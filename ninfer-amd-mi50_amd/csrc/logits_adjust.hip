@@ -47,86 +47,97 @@ __device__ __forceinline__ float penalised(float l, float p, unsigned count) {
 struct AdjustLds {
   // By token of the part: first what the list's entries say of it (0: nothing), then kListed and a 32-bit float.
   unsigned long long of[kAdjustPart];
-  // Entries of the list whose token lies in the part, as many as there is room for (the others are read where they are found):
-  // kEntry * the entry, from the list's first on, and the token. Then the tokens of these entries. Their memory leaves room for four
-  // blocks on a CU.
+  // Entries of the list whose token lies in the part, as many as leave room for four blocks' memory on a CU (the others are read
+  // where they are found): kEntry * the entry, from the list's first on, and the token.
   unsigned entry[kAdjustPart / 2 - 2];
-  int n_entries, n_listed;
+  int n_entries;
 };
 static_assert(sizeof(AdjustLds) <= 40960, "four blocks to a CU");
 constexpr unsigned long long kListed = 1ull << 63;
 constexpr unsigned kEntry = kAdjustPart, kMostEntries = kAdjustPart / 2 - 2;
 constexpr int kEntriesEach = (kMostEntries + kAdjustThreads - 1) / kAdjustThreads;
 
-// One list of the row, entries [first, end): `note(entry, token)` puts an entry of the part into l.of and says whether it is
-// its token's first; `value(token, what l.of has)` makes a float of that; `put(logit, float)` goes over the listed tokens' logits.
-// What an entry says is read, and the values are made, by as many threads as there are entries and tokens of the part: in the
-// loop over the list, or over the logits that a thread holds, nearly every wave would wait for those loads, and run a power and a
-// quotient in 64 bits, in every turn (256 rows of 151,936 tokens with 6,000 entries each, us: 181 so, 141 with the values alone
-// made so).
-template <typename Note, typename Value, typename Put>
-__device__ __forceinline__ bool apply_list(AdjustLds& l, const int* tokens, int first, int end, int t0, int n,
-                                           float (&v)[kAdjustQuads][4], Note note, Value value, Put put) {
+// Where `of` has a token: a thread's four neighbouring logits in four banks' worth of numbers side by side with its neighbours'.
+__device__ __forceinline__ int place_of(int token) { return (token & 3) * (kAdjustPart / 4) + (token >> 2); }
+
+// The tokens of a list's next entries, from e0 on a thread each; none for turns behind the list's end.
+__device__ __forceinline__ void load_tokens(int (&t)[kAdjustLists], const int* tokens, int e0, int end) {
+#pragma unroll
+  for (int u = 0; u < kAdjustLists; ++u) {
+    if (e0 + u * kAdjustThreads >= end) break;
+    t[u] = tokens[min(e0 + u * kAdjustThreads + (int)threadIdx.x, end - 1)];
+  }
+}
+
+// One list of the row, entries [first, end), `t` the tokens of the first ones, l.of all 0. `read(entry, token)` reads what an entry
+// says; `note(entry, token, that)` puts it into l.of and says whether it is its token's first; `value(what l.of has, that)`
+// makes a float for the token, in the thread that had its first entry; `again(token, what l.of has)` the same for tokens all of
+// whose entries found no room; `put(logit, float)` goes over the listed tokens' logits.
+// What entries say is read, and the values are made, by as many threads as there are entries and tokens of the part: in the loop over
+// the list, or over the logits that a thread holds, nearly every wave would wait for those loads, and run a power and a quotient
+// in 64 bits, in every turn (256 rows of 151,936 tokens with 6,000 entries each, us: 181 so, 141 with the values alone made so).
+template <typename Read, typename Note, typename Value, typename Again, typename Put>
+__device__ __forceinline__ bool apply_list(AdjustLds& l, int (&t)[kAdjustLists], const int* tokens, int first, int end, int t0, int n,
+                                           float (&v)[kAdjustQuads][4], Read read, Note note, Value value, Again again, Put put) {
   const int tid = threadIdx.x;
-  int t[kAdjustLists];
-  auto load = [&](int e0) {
-#pragma unroll
-    for (int u = 0; u < kAdjustLists; ++u) t[u] = tokens[min(e0 + u * kAdjustThreads, end - 1)];
-  };
-  load(first + tid);
-  __syncthreads();   // (the list before has been put)
-#pragma unroll
-  for (int i = 0; i < kAdjustPart / kAdjustThreads; ++i) l.of[i * kAdjustThreads + tid] = 0;
-  if (tid == 0) l.n_entries = l.n_listed = 0;
-  __syncthreads();
-  for (int e0 = first + tid; e0 < end; e0 += kAdjustLists * kAdjustThreads) {
-    if (e0 != first + tid) load(e0);
+  for (int e0 = first; e0 < end; e0 += kAdjustLists * kAdjustThreads) {
+    if (e0 != first) load_tokens(t, tokens, e0, end);
 #pragma unroll
     for (int u = 0; u < kAdjustLists; ++u) {
-      const int e = e0 + u * kAdjustThreads;
+      if (e0 + u * kAdjustThreads >= end) break;
+      const int e = e0 + u * kAdjustThreads + tid;
       const unsigned at = (unsigned)t[u] - (unsigned)t0;   // (ids outside the vocabulary fall outside every part)
       if (e < end && at < (unsigned)n) {
         const unsigned i = (unsigned)(e - first) < 0xffffffffu / kEntry ? atomicAdd(&l.n_entries, 1) : kMostEntries;
         if (i < kMostEntries) l.entry[i] = (unsigned)(e - first) * kEntry + at;
-        else note(e, (int)at);   // (its token, if this is its first entry, is found in `of`)
+        else note(e, (int)at, read(e, (int)at));
       }
     }
   }
   __syncthreads();
   const int entries = min(l.n_entries, (int)kMostEntries);
+  if (l.n_entries == 0 && (unsigned)(end - first) < 0xffffffffu / kEntry) return false;
   const bool all = l.n_entries <= (int)kMostEntries && (unsigned)(end - first) < 0xffffffffu / kEntry;
   unsigned mine[kEntriesEach];
+  decltype(read(0, 0)) that[kEntriesEach];
+  bool has[kEntriesEach];
 #pragma unroll
-  for (int u = 0; u < kEntriesEach; ++u) mine[u] = tid + u * kAdjustThreads < entries ? l.entry[tid + u * kAdjustThreads] : 0;
+  for (int u = 0; u < kEntriesEach; ++u) {
+    has[u] = tid + u * kAdjustThreads < entries;
+    if (has[u]) {
+      mine[u] = l.entry[tid + u * kAdjustThreads];
+      that[u] = read(first + (int)(mine[u] / kEntry), (int)(mine[u] % kEntry));
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kEntriesEach; ++u)
+    if (has[u]) has[u] = note(first + (int)(mine[u] / kEntry), (int)(mine[u] % kEntry), that[u]);
   __syncthreads();
 #pragma unroll
   for (int u = 0; u < kEntriesEach; ++u) {
-    const int at = mine[u] % kEntry;
-    if (tid + u * kAdjustThreads < entries && note(first + (int)(mine[u] / kEntry), at)) l.entry[atomicAdd(&l.n_listed, 1)] = at;
-  }
-  __syncthreads();
-  const int listed = l.n_listed;
-  for (int i = tid; i < listed; i += kAdjustThreads) {
-    const int at = l.entry[i];
-    l.of[at] = kListed | __float_as_uint(value(at, l.of[at]));
-  }
-  __syncthreads();
-  if (!all) {   // (tokens of other entries)
-    for (int at = tid; at < kAdjustPart; at += kAdjustThreads)
-      if (l.of[at] && !(l.of[at] & kListed)) l.of[at] = kListed | __float_as_uint(value(at, l.of[at]));
-    __syncthreads();
-  }
-  if (listed || !all) {
-#pragma unroll
-    for (int u = 0; u < kAdjustQuads; ++u) {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const unsigned long long x = l.of[(u * kAdjustThreads + tid) * 4 + c];
-        if (x) put(v[u][c], __uint_as_float((unsigned)x));
-      }
+    if (has[u]) {
+      const int at = (int)(mine[u] % kEntry);
+      unsigned long long& of = l.of[place_of(at)];
+      of = kListed | __float_as_uint(value(of, that[u]));
     }
   }
-  return listed > 0 || !all;
+  __syncthreads();
+  if (!all) {
+    for (int at = tid; at < kAdjustPart; at += kAdjustThreads) {
+      unsigned long long& of = l.of[place_of(at)];
+      if (of && !(of & kListed)) of = kListed | __float_as_uint(again(at, of));
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int u = 0; u < kAdjustQuads; ++u) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const unsigned long long x = l.of[c * (kAdjustPart / 4) + u * kAdjustThreads + tid];
+      if (x) put(v[u][c], __uint_as_float((unsigned)x));
+    }
+  }
+  return true;
 }
 
 __global__ __launch_bounds__(kAdjustThreads) void adjust_logits_kernel(const AdjustArgs a, int parts) {
@@ -144,6 +155,12 @@ __global__ __launch_bounds__(kAdjustThreads) void adjust_logits_kernel(const Adj
   const float rp = a.repetition ? a.repetition[r] : 1.f;
   const float freq = a.frequency ? a.frequency[r] : 0.f, pres = a.presence ? a.presence[r] : 0.f;
 
+  h0 = max(h0, 0), h1 = min(h1, a.n_hist), b0 = max(b0, 0), b1 = min(b1, a.n_bias);
+  if (rp == 1.f && freq == 0.f && pres == 0.f) h1 = h0;
+  // (the lists before the logits: a load is waited for after those that were asked for before it)
+  int ht[kAdjustLists], bt[kAdjustLists];
+  if (h1 > h0) load_tokens(ht, a.hist_tokens, h0, h1);
+  if (b1 > b0) load_tokens(bt, a.bias_tokens, b0, b1);
   float v[kAdjustQuads][4];
 #pragma unroll
   for (int u = 0; u < kAdjustQuads; ++u) {
@@ -167,26 +184,46 @@ __global__ __launch_bounds__(kAdjustThreads) void adjust_logits_kernel(const Adj
   }
 
   bool changed = masked || a.out != a.logits;
-  h0 = max(h0, 0), h1 = min(h1, a.n_hist), b0 = max(b0, 0), b1 = min(b1, a.n_bias);
-  if (h1 > h0 && (rp != 1.f || freq != 0.f || pres != 0.f)) {
-    changed |= apply_list(
-        l, a.hist_tokens, h0, h1, t0, n, v,
+  auto clear = [&] {
+#pragma unroll
+    for (int i = 0; i < kAdjustPart / kAdjustThreads; ++i) l.of[i * kAdjustThreads + tid] = 0;
+    if (tid == 0) l.n_entries = 0;
+    __syncthreads();
+  };
+  bool dirty = false;
+  if (h1 > h0) {
+    clear();
+    struct Said { unsigned count, generated; float logit; };
+    auto penalty = [&](float x, unsigned long long counts) {
+      if (rp != 1.f) x = penalised(x, rp, (unsigned)counts);
+      const unsigned g = (unsigned)(counts >> 32);
+      return g ? x - freq * (float)g - pres : x;
+    };
+    dirty = apply_list(
+        l, ht, a.hist_tokens, h0, h1, t0, n, v,
         [&](int e, int at) {
-          const unsigned c = max(a.hist_counts[e], 0), g = a.hist_generated ? max(a.hist_generated[e], 0) : 0;
-          return (c || g) && atomicAdd(&l.of[at], (unsigned long long)g << 32 | c) == 0;
+          return Said{(unsigned)max(a.hist_counts[e], 0), a.hist_generated ? (unsigned)max(a.hist_generated[e], 0) : 0u, row[at]};
         },
-        [&](int at, unsigned long long counts) {
-          float x = row[at];
-          if (rp != 1.f) x = penalised(x, rp, (unsigned)counts);
-          const unsigned g = (unsigned)(counts >> 32);
-          return g ? x - freq * (float)g - pres : x;
+        [&](int, int at, const Said& s) {
+          return (s.count || s.generated) && atomicAdd(&l.of[place_of(at)], (unsigned long long)s.generated << 32 | s.count) == 0;
         },
+        [&](unsigned long long counts, const Said& s) { return penalty(s.logit, counts); },
+        [&](int at, unsigned long long counts) { return penalty(row[at], counts); },
         [](float& logit, float x) { logit = x; });
+    changed |= dirty;
   }
   if (b1 > b0) {
+    if (h1 > h0) __syncthreads();   // (the list before has been put)
+    if (dirty || h1 <= h0) clear();
+    struct Said { int entry; float bias; };
     changed |= apply_list(
-        l, a.bias_tokens, b0, b1, t0, n, v,
-        [&](int e, int at) { return atomicMax(&l.of[at], (unsigned long long)(e - b0) + 1) == 0; },
+        l, bt, a.bias_tokens, b0, b1, t0, n, v,
+        [&](int e, int) { return Said{e, a.bias_values[e]}; },
+        [&](int e, int at, const Said&) { return atomicMax(&l.of[place_of(at)], (unsigned long long)(e - b0) + 1) == 0; },
+        [&](unsigned long long last, const Said& s) {
+          const int e = b0 + (int)last - 1;
+          return e == s.entry ? s.bias : a.bias_values[e];
+        },
         [&](int, unsigned long long last) { return a.bias_values[b0 + (int)last - 1]; },
         [](float& logit, float x) { logit += x; });
   }

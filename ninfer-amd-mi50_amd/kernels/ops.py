@@ -267,7 +267,7 @@ class _GatedSumArgs(ctypes.Structure):
 
 
 # Arguments of calls that a step makes many times, laid out by one call each (a ctypes structure costs the host three times as much)
-_ADAPTER_ARGS = struct.Struct("9Q3q6i5ii")    # x a b scale ranks row_adapter base out h | ldx ldb ldo | T K R S L N | first[5] | dtype
+_ADAPTER_ARGS = struct.Struct("9Q3q6i5i2i4x")   # x a b scale ranks row_adapter base out h | ldx ldb ldo | T K R S L N | first[5] | dtype single
 _ADJUST_ARGS = struct.Struct("14Q2q6i")       # logits out repetition presence frequency, histories, biases, masks mask_rows | ld ldo | R V n_hist n_bias n_masks vec
 _LOGPROB_ARGS = struct.Struct("9Qq4i")        # logits tokens logprob before best best_logprob sums counts keys | ld | R V top vec
 
@@ -2299,10 +2299,10 @@ class HipOps:
             first[i] = first[i - 1] + widths[i - 1]
         lib, stream, code = self.lib, self._stream_of(dev), _DT[dt]
         pa, p_b, ph = a.data_ptr(), b.data_ptr(), h.data_ptr()
-        # single rows are few-row tiles' work, however many rows there are behind them
+        # (single rows beside others: tiles of their own, where there are enough rows for two forms)
         for lo, hi in ((0, single_rows), (single_rows, t)) if 0 < single_rows < t and t >= 512 else ((0, t),):
             args = _ADAPTER_ARGS.pack(px + lo * ldx * size, pa, p_b, p_scale, p_ranks, p_rows + 4 * lo, pb + lo * ldb * size,
-                                      po + lo * ldo * size, ph + lo * slices * r * 4, ldx, ldb, ldo, hi - lo, k, r, slices, count, n, *first, code)
+                                      po + lo * ldo * size, ph + lo * slices * r * 4, ldx, ldb, ldo, hi - lo, k, r, slices, count, n, *first, code, hi <= single_rows)
             if lib.ninfer_adapter_add(args, stream):
                 self._ok(-1)
 

@@ -409,7 +409,7 @@ def test_the_library_refuses(lib):
     """Calls that end before anything is launched (no GPU here): sizes, strides, arrays that are missing."""
     from ninfer_amd.kernels.ops import _ADAPTER_ARGS, _ADJUST_ARGS, _LOGPROB_ARGS
     p = 1 << 20
-    fields = {_ADAPTER_ARGS: "x a b scale ranks row_adapter base out h ldx ldb ldo T K R S L N first dtype",
+    fields = {_ADAPTER_ARGS: "x a b scale ranks row_adapter base out h ldx ldb ldo T K R S L N first dtype single",
               _ADJUST_ARGS: "logits out repetition presence frequency hist_offsets hist_tokens hist_counts hist_generated bias_offsets bias_tokens "
                             "bias_values masks mask_rows ld ldo R V n_hist n_bias n_masks vec",
               _LOGPROB_ARGS: "logits tokens logprob before best best_logprob sums counts keys ld R V top vec"}
