@@ -68,18 +68,25 @@ template <> struct Frag<float> {
   }
 };
 
-// Numbers [at, at + kLane) of a row of `n`, 0 behind its end (nothing is read there).
-template <bool VEC, typename T>
+// 16 bytes by one load or store, which ask for addresses that are multiples of 4.
+struct __attribute__((packed, aligned(4))) Sixteen { uint4 v; };
+__device__ __forceinline__ uint4 load_16_bytes(const void* p) { return ((const Sixteen*)p)->v; }
+__device__ __forceinline__ void store_16_bytes(void* p, uint4 v) { ((Sixteen*)p)->v = v; }
+
+// Numbers [at, at + kLane) of a row of `n`, 0 behind its end (nothing is read there), one by one.
+template <typename T>
+__device__ __forceinline__ uint4 load_single(const T* row, int at, int n) {
+  T e[Frag<T>::kLane];
+#pragma unroll
+  for (int i = 0; i < Frag<T>::kLane; ++i) e[i] = at + i < n ? row[at + i] : from_f32<T>(0.f);
+  uint4 v;
+  __builtin_memcpy(&v, e, 16);
+  return v;
+}
+template <typename T>
 __device__ __forceinline__ Frag<T> load_frag(const T* row, int at, int n) {
   Frag<T> f;
-  if (VEC && at + Frag<T>::kLane <= n) {
-    f.v = *(const decltype(f.v)*)(row + at);
-  } else {
-    T e[Frag<T>::kLane];
-#pragma unroll
-    for (int i = 0; i < Frag<T>::kLane; ++i) e[i] = at + i < n ? row[at + i] : from_f32<T>(0.f);
-    __builtin_memcpy(&f.v, e, sizeof(f.v));
-  }
+  f.v = __builtin_bit_cast(decltype(f.v), load_single(row, at, n));
   return f;
 }
 
@@ -111,7 +118,7 @@ struct TileAdapters {
 // are fewer). By the whole block of WAVES waves: 64 tiles of 32 rows at a time, their numbers of further adapters in `counts` [64].
 template <int WAVES>
 __device__ int find_further(const AdapterArgs& a, int u, int* counts, int& tile) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, tiles = (a.T + 31) / 32;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tiles = (a.T + 31) / 32;
   for (int base = 0; base < tiles; base += 64) {
     int of[32 / WAVES];   // a wave's pairs of tiles, a row a lane
 #pragma unroll
@@ -158,21 +165,25 @@ __device__ __forceinline__ bool place_of(int b, bool near, int groups, int total
   return b < total;
 }
 
-// The 16 bytes at number `k` of a row of whole such pieces, its numbers from `rank` on as 0 (whatever they are).
+// All bits of the first `count` of 16 bytes' numbers.
 template <typename T>
-__device__ __forceinline__ uint4 load_piece(const T* row, int k, int rank) {
-  if (k >= rank) return make_uint4(0, 0, 0, 0);
-  uint4 v = *(const uint4*)(row + k);
-  const int left = rank - k;   // numbers that count
-  if (left < Frag<T>::kLane) {
-    uint32_t* u = (uint32_t*)&v;
+__device__ __forceinline__ uint4 first_numbers(int count) {
+  uint32_t u[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int bits = (left - i * (4 / (int)sizeof(T))) * 8 * (int)sizeof(T);
-      u[i] = bits >= 32 ? u[i] : bits <= 0 ? 0u : u[i] & ((1u << bits) - 1);
-    }
+  for (int i = 0; i < 4; ++i) {
+    const int bits = (count - i * (4 / (int)sizeof(T))) * 8 * (int)sizeof(T);
+    u[i] = bits >= 32 ? ~0u : bits <= 0 ? 0u : (1u << bits) - 1;
   }
-  return v;
+  return make_uint4(u[0], u[1], u[2], u[3]);
+}
+
+// The 16 bytes at number `k` of a row of `n` numbers of which `rank` count: the others are 0, whatever they are.
+template <typename T>
+__device__ __forceinline__ uint4 load_piece(const T* row, int k, int rank, int n) {
+  if (k >= rank) return make_uint4(0, 0, 0, 0);
+  if (k + Frag<T>::kLane > n) return load_single(row, k, rank);
+  const uint4 v = load_16_bytes(row + k), keep = first_numbers<T>(rank - k);
+  return make_uint4(v.x & keep.x, v.y & keep.y, v.z & keep.z, v.w & keep.w);
 }
 
 // Between a wave's writes into its own shared memory and its lanes' reads of each other's: the memory itself keeps a wave's order.
@@ -191,26 +202,27 @@ __device__ __forceinline__ int place8(int row, int piece) { return row * 8 + (pi
 __device__ __forceinline__ int place4(int row, int piece) { return row * 4 + (piece ^ (row >> 2)); }
 
 // h of 16 RT rows and 16 CT columns.
-template <typename T, int RT, int CT, bool VEC>
+enum Rows { kSingle, kWhole, kRest };   // numbers one by one; 16 bytes at a time, rows of whole steps, or with a rest behind them
+
+template <typename T, int RT, int CT, Rows ROWS>
 __global__ __launch_bounds__(kShrinkWaves * 64, RT == 1 ? 4 : 2) void adapter_shrink_kernel(const AdapterArgs a, int groups, int total, int more) {
   constexpr int F = RT + CT, kLane = Frag<T>::kLane, kStep = 8 * kLane;   // (a step: 128 bytes of each row, two products)
-  constexpr int kDepth = F <= 2 ? 4 : 2;   // steps on their way
+  constexpr int kDepth = RT == 1 && ROWS == kWhole ? 3 : 2;   // steps on their way
   constexpr int kStage = kShrinkWaves * F * 128, kPart = kShrinkWaves * RT * CT * 64;
   __shared__ uint4 lds[kStage > kPart ? kStage : kPart];
   // `more` > 0: tiles have a block for their first adapters only, and as many more look for the further ones; else as in the other
   // kernel every gridDim.y'th.
-  const int first_blocks = gridDim.x - more;
-  int further = (int)blockIdx.x - first_blocks, tile_at = 0, group = 0, pass = blockIdx.y;
+  int further = RT > 1 ? (int)blockIdx.x - (int)(gridDim.x - more) : -1, tile_at = 0, group = 0, pass = blockIdx.y;
   if (further < 0 && !place_of(blockIdx.x, RT > 1, groups, total, tile_at, group)) return;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, quad = lane >> 4, m = lane & 15, C = a.S * a.R;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quad = lane >> 4, m = lane & 15, C = a.S * a.R;
   const int steps = (a.K + kStep - 1) / kStep;
   for (bool once = false;; once = true) {
     if (once) {
-      if (more && further < 0) return;
+      if (RT > 1 && more && further < 0) return;
       pass += gridDim.y;
       __syncthreads();   // (the memory is the next products')
     }
-    if (further >= 0) {
+    if (RT > 1 && further >= 0) {
       pass = find_further<kShrinkWaves>(a, further / groups, (int*)lds, tile_at);
       if (pass < 0) return;
       group = further % groups;
@@ -247,41 +259,42 @@ __global__ __launch_bounds__(kShrinkWaves * 64, RT == 1 ? 4 : 2) void adapter_sh
         for (int ct = 0; ct < CT; ++ct) acc[rt][ct] = Frag<T>::mma(f[rt], f[RT + ct], acc[rt][ct]);
     };
     // wave w takes the steps w, w + 8, ..
-    if constexpr (VEC) {
+    if constexpr (ROWS != kSingle) {
       uint4* stage = lds + w * (F * 128);
+      const int r = lane >> 3, c = lane & 7, whole = a.K / kStep;
       const T* from[F][2];
       uint4 next[kDepth][F][2];
 #pragma unroll
       for (int f = 0; f < F; ++f)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) from[f][i] = row_of(f, i * 8 + (lane >> 3)) + (lane & 7) * kLane;
+        for (int i = 0; i < 2; ++i) from[f][i] = row_of(f, i * 8 + r) + c * kLane;
       auto load = [&](uint4 (&to)[F][2], int st) {
-        if ((st + 1) * kStep <= a.K) {
 #pragma unroll
-          for (int f = 0; f < F; ++f)
+        for (int f = 0; f < F; ++f)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) to[f][i] = *(const uint4*)(from[f][i] + st * kStep);
-        } else {
-          const bool in = st * kStep + (lane & 7) * kLane < a.K;
-#pragma unroll
-          for (int f = 0; f < F; ++f)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) to[f][i] = in ? *(const uint4*)(from[f][i] + st * kStep) : make_uint4(0, 0, 0, 0);
-        }
+          for (int i = 0; i < 2; ++i) to[f][i] = load_16_bytes(from[f][i] + st * kStep);
       };
 #pragma unroll
       for (int d = 0; d < kDepth; ++d)
-        if (w + d * kShrinkWaves < steps) load(next[d], w + d * kShrinkWaves);
+        if (w + d * kShrinkWaves < whole) load(next[d], w + d * kShrinkWaves);
       for (int st0 = w; st0 < steps; st0 += kDepth * kShrinkWaves) {
 #pragma unroll
         for (int d = 0; d < kDepth; ++d) {
           const int st = st0 + d * kShrinkWaves;
           if (st >= steps) break;
+          if (ROWS == kWhole || st < whole) {
 #pragma unroll
-          for (int f = 0; f < F; ++f)
+            for (int f = 0; f < F; ++f)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) stage[f * 128 + place8(i * 8 + (lane >> 3), lane & 7)] = next[d][f][i];
-          if (st + kDepth * kShrinkWaves < steps) load(next[d], st + kDepth * kShrinkWaves);
+              for (int i = 0; i < 2; ++i) stage[f * 128 + place8(i * 8 + r, c)] = next[d][f][i];
+            if (st + kDepth * kShrinkWaves < whole) load(next[d], st + kDepth * kShrinkWaves);
+          } else {   // (the rest of the rows)
+#pragma unroll 1
+            for (int f = 0; f < F; ++f)
+#pragma unroll 1
+              for (int i = 0; i < 2; ++i)
+                stage[f * 128 + place8(i * 8 + r, c)] = load_piece(row_of(f, i * 8 + r), st * kStep + c * kLane, a.K, a.K);
+          }
           wave_fence();
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
@@ -299,7 +312,7 @@ __global__ __launch_bounds__(kShrinkWaves * 64, RT == 1 ? 4 : 2) void adapter_sh
         for (int k = st * kStep + quad * kLane; k < (st + 1) * kStep; k += 4 * kLane) {
           Frag<T> f[F];
 #pragma unroll
-          for (int i = 0; i < F; ++i) f[i] = load_frag<false>(row_of(i, m), k, a.K);
+          for (int i = 0; i < F; ++i) f[i] = load_frag(row_of(i, m), k, a.K);
           multiply(f);
         }
       }
@@ -363,7 +376,7 @@ __device__ __forceinline__ bool expand_tile(const AdapterArgs& a, int t0, int se
 #pragma unroll
       for (int i = 0; i < 16 / kRows; ++i) {
         const int r = rt * 16 + i * kRows + lane / kCols;
-        if (rows >> r & 1) was[rt][i] = *(const uint4*)(base + (t0 + r) * a.ldb + lane % kCols * kEach);
+        if (rows >> r & 1) was[rt][i] = load_16_bytes(base + (t0 + r) * a.ldb + lane % kCols * kEach);
       }
   };
   auto store = [&](int rt, unsigned long long rows, float scale, const float* tile_) {   // tile_: rows of kRow floats, or null: 0
@@ -380,7 +393,7 @@ __device__ __forceinline__ bool expand_tile(const AdapterArgs& a, int t0, int se
         }
         uint4 v;
         __builtin_memcpy(&v, e, 16);
-        *(uint4*)(out + (t0 + r) * a.ldo + lane % kCols * kEach) = v;
+        store_16_bytes(out + (t0 + r) * a.ldo + lane % kCols * kEach, v);
       }
     } else {
 #pragma unroll 1
@@ -420,15 +433,22 @@ __device__ __forceinline__ bool expand_tile(const AdapterArgs& a, int t0, int se
   for (int k0 = 0; k0 < rank; k0 += kStep) {
     if constexpr (VEC) {
       const int k = k0 + (lane & 3) * kLane, r = lane >> 2;
-      uint4 now[4 + RT * kTerms<T>];
+      auto row_of = [&](int f) { return f < 4 ? brow(f, r) : hrow((f - 4) / kTerms<T>, r) + (f - 4) % kTerms<T> * plane; };
+      if (k0 + kStep <= a.R || a.R % kLane == 0) {   // (16 bytes that begin in a row end in it)
+        uint4 now[4 + RT * kTerms<T>];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) now[j] = load_piece(brow(j, r), k, rank);
+        for (int f = 0; f < 4 + RT * kTerms<T>; ++f) now[f] = k < rank ? load_16_bytes(row_of(f) + k) : make_uint4(0, 0, 0, 0);
+        if (k0 + kStep > rank) {
+          const uint4 keep = first_numbers<T>(rank - k);
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
+          for (int f = 0; f < 4 + RT * kTerms<T>; ++f) now[f].x &= keep.x, now[f].y &= keep.y, now[f].z &= keep.z, now[f].w &= keep.w;
+        }
 #pragma unroll
-        for (int x = 0; x < kTerms<T>; ++x) now[4 + rt * kTerms<T> + x] = load_piece(hrow(rt, r) + x * plane, k, rank);
-#pragma unroll
-      for (int f = 0; f < 4 + RT * kTerms<T>; ++f) stage[f * 64 + place4(r, lane & 3)] = now[f];
+        for (int f = 0; f < 4 + RT * kTerms<T>; ++f) stage[f * 64 + place4(r, lane & 3)] = now[f];
+      } else {
+#pragma unroll 1
+        for (int f = 0; f < 4 + RT * kTerms<T>; ++f) stage[f * 64 + place4(r, lane & 3)] = load_piece(row_of(f), k, rank, a.R);
+      }
       wave_fence();
       Frag<T> bf[4];
 #pragma unroll
@@ -447,12 +467,12 @@ __device__ __forceinline__ bool expand_tile(const AdapterArgs& a, int t0, int se
       const int k = k0 + quad * kLane;
       Frag<T> bf[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) bf[j] = load_frag<false>(brow(j, m), k, rank);
+      for (int j = 0; j < 4; ++j) bf[j] = load_frag(brow(j, m), k, rank);
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
         for (int x = 0; x < kTerms<T>; ++x) {
-          const Frag<T> hf = load_frag<false>(hrow(rt, m) + x * plane, k, rank);
+          const Frag<T> hf = load_frag(hrow(rt, m) + x * plane, k, rank);
 #pragma unroll
           for (int j = 0; j < 4; ++j) acc[rt][j] = Frag<T>::mma(bf[j], hf, acc[rt][j]);
         }
@@ -473,16 +493,16 @@ __device__ __forceinline__ bool expand_tile(const AdapterArgs& a, int t0, int se
 
 // Four waves take neighbouring columns. `more`: as in the other kernel.
 template <typename T, int RT, bool VEC>
-__global__ __launch_bounds__(kExpandWaves * 64) void adapter_expand_kernel(const AdapterArgs a, int sets, int groups, int total, int more,
+__global__ __launch_bounds__(kExpandWaves * 64, RT == 1 ? 4 : 3) void adapter_expand_kernel(const AdapterArgs a, int sets, int groups, int total, int more,
                                                                            bool vec_out) {
   constexpr int kStage = (4 + RT * kTerms<T>) * 64, kTile = 16 * kRow / 4;
   __shared__ uint4 lds[kExpandWaves][kStage > kTile ? kStage : kTile];
   __shared__ int counts[64];
-  int further = (int)blockIdx.x < more ? (int)blockIdx.x : -1, tile = 0, group = 0, pass = blockIdx.y;
+  int further = RT > 1 && (int)blockIdx.x < more ? (int)blockIdx.x : -1, tile = 0, group = 0, pass = blockIdx.y;
   if (further < 0 && !place_of(blockIdx.x - more, RT > 1, groups, total, tile, group)) return;
-  const int wave = threadIdx.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   for (;; pass += gridDim.y) {
-    if (further >= 0) {
+    if (RT > 1 && further >= 0) {
       pass = find_further<kExpandWaves>(a, further / groups, counts, tile);
       if (pass < 0) return;
       group = further % groups;
@@ -506,28 +526,27 @@ static dim3 grid_of(const AdapterArgs& a, int total, int* more) {
 
 template <typename T, int RT, int CT>
 static void shrink(const AdapterArgs& a, hipStream_t stream) {
-  constexpr int kLane = Frag<T>::kLane;
   const int groups = (a.S * a.R + CT * 16 - 1) / (CT * 16), total = (a.T + 16 * RT - 1) / (16 * RT) * groups;
   int more = 0;
   const dim3 grid = grid_of<RT>(a, total, &more);
-  const bool vec = (uintptr_t)a.x % 16 == 0 && (uintptr_t)a.a % 16 == 0 && a.K % kLane == 0 && a.ldx % kLane == 0;
-  if (vec) adapter_shrink_kernel<T, RT, CT, true><<<grid, kShrinkWaves * 64, 0, stream>>>(a, groups, total, more);
-  else adapter_shrink_kernel<T, RT, CT, false><<<grid, kShrinkWaves * 64, 0, stream>>>(a, groups, total, more);
+  const bool vec = (uintptr_t)a.x % 4 == 0 && (uintptr_t)a.a % 4 == 0 && a.K * sizeof(T) % 4 == 0 && a.ldx * sizeof(T) % 4 == 0;
+  if (!vec) adapter_shrink_kernel<T, RT, CT, kSingle><<<grid, kShrinkWaves * 64, 0, stream>>>(a, groups, total, more);
+  else if (a.K % (8 * Frag<T>::kLane)) adapter_shrink_kernel<T, RT, CT, kRest><<<grid, kShrinkWaves * 64, 0, stream>>>(a, groups, total, more);
+  else adapter_shrink_kernel<T, RT, CT, kWhole><<<grid, kShrinkWaves * 64, 0, stream>>>(a, groups, total, more);
 }
 
 template <typename T, int RT>
 static void expand(const AdapterArgs& a, hipStream_t stream) {
-  constexpr int kLane = Frag<T>::kLane;
   int sets = 0;
-  bool vec_out = (uintptr_t)a.out % 16 == 0 && (uintptr_t)a.base % 16 == 0 && a.ldo * sizeof(T) % 16 == 0 && a.ldb * sizeof(T) % 16 == 0;
+  bool vec_out = (uintptr_t)a.out % 4 == 0 && (uintptr_t)a.base % 4 == 0 && a.ldo * sizeof(T) % 4 == 0 && a.ldb * sizeof(T) % 4 == 0;
   for (int s = 0; s < a.S; ++s) {
     sets += (a.first[s + 1] - a.first[s] + 63) / 64;
-    vec_out &= a.first[s] * sizeof(T) % 16 == 0;
+    vec_out &= a.first[s] * sizeof(T) % 4 == 0;
   }
   const int groups = (sets + kExpandWaves - 1) / kExpandWaves, total = (a.T + 16 * RT - 1) / (16 * RT) * groups;
   int more = 0;
   const dim3 grid = grid_of<RT>(a, total, &more);
-  const bool vec = (uintptr_t)a.b % 16 == 0 && a.R % kLane == 0;
+  const bool vec = (uintptr_t)a.b % 4 == 0 && a.R * sizeof(T) % 4 == 0;
   if (vec) adapter_expand_kernel<T, RT, true><<<grid, kExpandWaves * 64, 0, stream>>>(a, sets, groups, total, more, vec_out);
   else adapter_expand_kernel<T, RT, false><<<grid, kExpandWaves * 64, 0, stream>>>(a, sets, groups, total, more, vec_out);
 }
