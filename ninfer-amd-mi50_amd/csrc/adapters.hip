@@ -551,12 +551,16 @@ static void expand(const AdapterArgs& a, hipStream_t stream) {
   else adapter_expand_kernel<T, RT, false><<<grid, kExpandWaves * 64, 0, stream>>>(a, sets, groups, total, more, vec_out);
 }
 
-// Rows from which tiles of 32 are the faster ones, unless every row has an adapter of its own.
-constexpr int kManyRows = 512;
+// Blocks of 32 rows and 64 columns of the first product from which these are the faster ones: blocks of 16 by 16 are many more. us so
+// and in blocks of 16 by 16, one adapter a tile: bfloat16, 3 x 64 columns of 2,048, 384 rows 21 and 16, 512 (48 blocks) 15.8 and 16.7,
+// 2,048 26 and 38; 64 columns, 1,024 rows (32) 14.5 and 12.8, 2,048 (64) 16 and 19; 32-bit, 3 x 64 columns, 1,024 rows (96) 48 and 43,
+// 2,048 (192) 65 and 68. Rows that each have an adapter of their own never: 512 of eight adapters in turn 95 and 69.
+template <typename T> constexpr int kManyBlocks = sizeof(T) == 2 ? 48 : 192;
 
 template <typename T>
 static void launch(const AdapterArgs& a, hipStream_t stream) {
-  if (a.T >= kManyRows && !a.single) {
+  const long long blocks = (a.T + 31ll) / 32 * ((a.S * a.R + 63) / 64);
+  if (blocks >= kManyBlocks<T> && !a.single) {
     shrink<T, 2, 4>(a, stream);
     expand<T, 2>(a, stream);
   } else {
@@ -581,8 +585,10 @@ extern "C" int ninfer_adapter_add(const AdapterArgs* args, hipStream_t stream) {
   NINFER_REQUIRE(a.x && a.a && a.b && a.scale && a.ranks && a.row_adapter && a.base && a.out && a.h, "adapter_add: a required array is null");
   NINFER_REQUIRE(a.ldx >= a.K && a.ldb >= a.N && a.ldo >= a.N, "adapter_add: a row stride is less than the row");
   NINFER_REQUIRE(a.base != a.out || a.ldb == a.ldo, "adapter_add: in place with two row strides");
-  NINFER_REQUIRE((long long)a.T * a.S * a.R <= 0x7fffffff && (long long)a.T * (a.N / 64 + 8) / 16 <= 0x7fffffff,
-                 "adapter_add: %d rows are too many", a.T);
+  // (threads of a grid's x, in blocks of 16 rows: 512 for 16 columns of h, 64 for 64 of out)
+  const long long tiles = (a.T + 15ll) / 16;
+  NINFER_REQUIRE(a.S * (long long)a.R <= 0x7fffffff && tiles * ((a.S * a.R + 15ll) / 16) * 512 <= 0x7fffffffll &&
+                     tiles * (a.N / 64 + 8ll) * 64 <= 0x7fffffffll, "adapter_add: %d rows are too many", a.T);
   NINFER_REQUIRE(a.dtype == kF32 || a.dtype == kBF16, "adapter_add: dtype %d", a.dtype);
   if (a.dtype == kBF16) launch<bf16>(a, stream);
   else launch<float>(a, stream);

@@ -263,7 +263,7 @@ extern "C" int ninfer_adjust_logits(const AdjustArgs* args, hipStream_t stream) 
   NINFER_REQUIRE(!a.bias_offsets || a.n_bias == 0 || (a.bias_tokens && a.bias_values), "adjust_logits: biases without tokens or values");
   NINFER_REQUIRE(!a.mask_rows || a.n_masks == 0 || a.masks, "adjust_logits: rows name masks that are not given");
   const int parts = (a.V + kAdjustPart - 1) / kAdjustPart;
-  NINFER_REQUIRE((long long)parts * a.R <= 0x7fffffff, "adjust_logits: %d rows are too many", a.R);
+  NINFER_REQUIRE((long long)parts * a.R <= 0xffffffffll / kAdjustThreads, "adjust_logits: %d rows are too many", a.R);
   a.vec = row_aligned(a.logits) && row_aligned(a.out) && a.ld % 4 == 0 && a.ldo % 4 == 0;
   adjust_logits_kernel<<<parts * a.R, kAdjustThreads, 0, stream>>>(a, parts);
   NINFER_LAUNCH_CHECK();

@@ -305,7 +305,7 @@ extern "C" int ninfer_token_logprobs(const LogprobArgs* args, void* scratch, hip
   NINFER_REQUIRE(a.tokens || a.top > 0, "token_logprobs: nothing is asked for");
   const int parts = (a.V + kLpPart - 1) / kLpPart;
   const long long blocks = (long long)parts * a.R;
-  NINFER_REQUIRE(blocks <= 0x7fffffff, "token_logprobs: %d rows are too many", a.R);
+  NINFER_REQUIRE(blocks <= 0xffffffffll / kLpThreads && a.R <= 0xffffffffll / kLpJoinThreads, "token_logprobs: %d rows are too many", a.R);
   a.vec = row_aligned(a.logits) && a.ld % 4 == 0;
   char* at = (char*)scratch;
   a.sums = (float2*)at;

@@ -142,7 +142,7 @@ class ModelRunner:
             self.adapters.hold(name)
 
     def let_go_adapter(self, name: Optional[str]) -> None:
-        if name is not None:
+        if name is not None and self.adapters is not None:   # (None once the runner is released)
             self.adapters.let_go(name)
 
     def release(self) -> None:

@@ -2282,6 +2282,8 @@ class HipOps:
         p_rows = self._flat(row_adapter, torch.int32, t, dev, "adapter_add: row_adapter")
         if not 0 <= single_rows <= t:
             raise KernelError(f"adapter_add: {single_rows} single rows of {t}")
+        if self._held is not None:
+            raise KernelError("adapter_add: inside together(), where products have not been launched")
         if t == 0:
             return
         px, po = x.data_ptr(), out.data_ptr()

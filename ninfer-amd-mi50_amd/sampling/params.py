@@ -12,6 +12,8 @@ import math
 from dataclasses import dataclass
 from typing import Dict, Optional
 
+_MOST = 3.4028234663852886e38   # the largest 32-bit float
+
 
 @dataclass
 class SamplingParams:
@@ -29,12 +31,12 @@ class SamplingParams:
     def check(self, vocab: int, most_listed: int) -> None:
         """ValueError for what no row of `vocab` logits can be asked for."""
         for name in ("presence_penalty", "frequency_penalty"):
-            if not math.isfinite(getattr(self, name)):
+            if not abs(getattr(self, name)) <= _MOST:
                 raise ValueError(f"{name} must be finite, is {getattr(self, name)}")
         for token, bias in (self.logit_bias or {}).items():
             if not 0 <= int(token) < vocab:
                 raise ValueError(f"logit_bias names token {token}, the vocabulary is [0, {vocab})")
-            if math.isnan(bias) or bias == math.inf:
+            if not (abs(bias) <= _MOST or bias == -math.inf):
                 raise ValueError(f"logit_bias of token {token} is {bias}")
         if self.logprobs is not None and not 0 <= self.logprobs <= min(most_listed, vocab):
             raise ValueError(f"logprobs must be in [0, {min(most_listed, vocab)}], is {self.logprobs}")

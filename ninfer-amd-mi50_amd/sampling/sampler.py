@@ -136,7 +136,8 @@ class SampleRow:
         self.params = params
         self.allowed = allowed
         # (a change of logits beyond the repetition penalty, which the sampling kernels apply themselves)
-        self.changes = allowed is not None or bool(params.presence_penalty or params.frequency_penalty or params.logit_bias)
+        self.changes = (allowed is not None or params.presence_penalty != 0.0 or params.frequency_penalty != 0.0
+                        or bool(params.logit_bias))
         self.history = history if isinstance(history, History) else History(
             t for t, c in dict(history).items() for _ in range(c))
         self.key = key
@@ -267,15 +268,15 @@ class Sampler:
 
     def sample(self, logits: torch.Tensor, rows: Sequence[SampleRow]) -> List[int]:
         """One token per row of `logits` [R, vocab]."""
-        if not any(row.changes for row in rows):
+        if True not in [row.changes for row in rows]:
             return self._sample(logits, rows)
         logits, slot = self.adjusted(logits, rows)
-        tokens = self._sample(logits, rows)
+        tokens = self._sample(logits, rows, changed=True)
         if slot is not None:
             self._free.append(slot)
         return tokens
 
-    def _sample(self, logits: torch.Tensor, rows: Sequence[SampleRow]) -> List[int]:
+    def _sample(self, logits: torch.Tensor, rows: Sequence[SampleRow], changed: bool = False) -> List[int]:
         r = len(rows)
         assert logits.shape[0] == r
         # Everything the kernel needs of the rows travels in one array and one copy: four
@@ -283,8 +284,8 @@ class Sampler:
         # and counts. (Copies queue behind the step that makes the logits, one after the other:
         # every further one would add its latency to the step.)
         temps, tops, penalties, top_ks = zip(*map(_OPTIONS, (row.params for row in rows))) if r else ((),) * 4
-        # (rows whose logits were changed have had their penalty)
-        penalties = [1.0 if row.changes else penalty for row, penalty in zip(rows, penalties)]
+        if changed:   # (rows whose logits were changed have had their penalty)
+            penalties = [1.0 if row.changes else penalty for row, penalty in zip(rows, penalties)]
         listed = [len(row.history) if penalty != 1.0 else 0 for row, penalty in zip(rows, penalties)]
         n_pen = sum(listed)
         o = 5 * r

@@ -70,7 +70,7 @@ def test_adapters(ops, dtype, t, k, widths, r, count, kind):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("t,count", [(512, 1), (600, 70), (2061, 40), (5000, 3)])
+@pytest.mark.parametrize("t,count", [(512, 1), (600, 70), (1537, 9), (2061, 40), (6200, 3)])
 @pytest.mark.parametrize("kind", ["one", "mixed", "portions", "last"])
 def test_adapters_of_many_rows(ops, dtype, t, count, kind):
     """Tiles of one adapter, of as many as rows, and a step of which only the last rows have any."""
@@ -199,6 +199,8 @@ def test_adapters_refusals(ops):
     for single in (-1, 5):
         with pytest.raises(KernelError, match="single rows"):
             ops.adapter_add(x, a, b, scale, ranks, (32, 32), rows, base, single_rows=single)
+    with pytest.raises(KernelError, match="together"), ops.together():
+        ops.adapter_add(x, a, b, scale, ranks, (32, 32), rows, base)
     assert torch.equal(base, before)
     ops.adapter_add(x[:0], a, b, scale, ranks, (32, 32), rows[:0], base[:0])   # no rows: nothing to do
 
