@@ -194,16 +194,17 @@ __device__ __forceinline__ void wave_fence() {
 
 // Rows on their way to the matrix units pass through shared memory of the wave: there a lane needs 16 bytes of row `lane % 16`, and
 // such loads, whose neighbouring lanes read different rows, cost the cache four times what loads of whole lines do (2,055 rows of
-// 3,584 numbers: 42 us, of which 4 are left). 16 rows of 128 bytes, eight pieces each: piece c of row r lies at 8 r + (c ^ r / 2),
+// 3,584 numbers, the first product: 42 us so, 18 through shared memory; the second 26 and 17). 16 rows of 128 bytes, eight pieces each: piece c of row r lies at 8 r + (c ^ r / 2),
 // so that sixteen rows' pieces of one number lie in different banks. A lane loads (and puts) piece lane % 8 of rows lane / 8 and
 // lane / 8 + 8.
 __device__ __forceinline__ int place8(int row, int piece) { return row * 8 + (piece ^ (row >> 1)); }
 // ... and of 64 bytes, four pieces each.
 __device__ __forceinline__ int place4(int row, int piece) { return row * 4 + (piece ^ (row >> 2)); }
 
-// h of 16 RT rows and 16 CT columns.
-enum Rows { kSingle, kWhole, kRest };   // numbers one by one; 16 bytes at a time, rows of whole steps, or with a rest behind them
+// How rows are read: number by number; 16 bytes at a time, rows of whole steps, or with a rest behind them.
+enum Rows { kSingle, kWhole, kRest };
 
+// h of 16 RT rows and 16 CT columns.
 template <typename T, int RT, int CT, Rows ROWS>
 __global__ __launch_bounds__(kShrinkWaves * 64, RT == 1 ? 4 : 2) void adapter_shrink_kernel(const AdapterArgs a, int groups, int total, int more) {
   constexpr int F = RT + CT, kLane = Frag<T>::kLane, kStep = 8 * kLane;   // (a step: 128 bytes of each row, two products)
