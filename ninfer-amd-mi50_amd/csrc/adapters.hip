@@ -5,7 +5,7 @@
 //   h[t, s, i] = sum_k A[g, s R + i, k] x[t, k]                       i < ranks[g]
 //   out[t, c] = base[t, c] + scale[g] sum_i B[g, c, i] h[t, s(c), i]
 //
-// Two launches: all slices' h, kept in 32 bits (scratch [T, S R]), then the columns. Both give a block
+// Two launches, but for few rows of small rank: all slices' h, kept in 32 bits (scratch [T, S R]), then the columns. Both give a block
 // tiles of 16 or 32 rows on the matrix units, whatever adapters these rows have: the products of a tile and
 // one of its adapters are a block's work, the rows of others ride along unwritten. Rows of a request are
 // neighbours, so a tile of a prompt's portion has one adapter, as a rule; a tile of single rows may have as
@@ -42,7 +42,7 @@ struct AdapterArgs {
   int single;            // the rows are of different requests each
 };
 
-constexpr int kShrinkWaves = 8;
+constexpr int kWaves = 8;
 constexpr int kExpandWaves = 4;
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -110,6 +110,15 @@ struct TileAdapters {
     left &= ~rows;
     rank = a.L <= 64 ? __builtin_amdgcn_readlane(ranks, g) : a.ranks[g];
     rank = min(max(rank, 0), a.R);
+    return g;
+  }
+  // The one after `pass` others; -1: there is none.
+  __device__ __forceinline__ int at(const AdapterArgs& a, int pass, unsigned long long& rows, int& rank) {
+    int g = -1;
+    for (int i = 0; left && i <= pass; ++i) {
+      const int one = next(a, rows, rank);
+      if (i == pass) g = one;
+    }
     return g;
   }
 };
@@ -204,19 +213,126 @@ __device__ __forceinline__ int place4(int row, int piece) { return row * 4 + (pi
 // How rows are read: number by number; 16 bytes at a time, rows of whole steps, or with a rest behind them.
 enum Rows { kSingle, kWhole, kRest };
 
+// Products of the 16 RT rows row_of(f, 0 .. 15), f < RT, with the 16 CT that follow: this wave's part of the sums over k, the steps
+// w, w + 8, .. of the block's eight waves. `lds`: memory of the block for all its rows on their way.
+template <typename T, int RT, int CT, Rows ROWS, typename RowOf>
+__device__ __forceinline__ void products(int K, uint4* lds, f32x4 (&acc)[RT][CT], RowOf row_of) {
+  constexpr int F = RT + CT, kLane = Frag<T>::kLane, kStep = 8 * kLane;   // (a step: 128 bytes of each row, two products)
+  constexpr int kDepth = RT == 1 && CT == 1 && ROWS == kWhole ? 3 : 2;    // steps on their way
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quad = lane >> 4, m = lane & 15;
+  const int steps = (K + kStep - 1) / kStep;
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) acc[rt][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto multiply = [&](const Frag<T> (&f)[F]) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) acc[rt][ct] = Frag<T>::mma(f[rt], f[RT + ct], acc[rt][ct]);
+  };
+  if constexpr (ROWS != kSingle) {
+    uint4* stage = lds + w * (F * 128);
+    const int r = lane >> 3, c = lane & 7, whole = K / kStep;
+    const T* from[F][2];
+    uint4 next[kDepth][F][2];
+#pragma unroll
+    for (int f = 0; f < F; ++f)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) from[f][i] = row_of(f, i * 8 + r) + c * kLane;
+    auto load = [&](uint4 (&to)[F][2], int st) {
+#pragma unroll
+      for (int f = 0; f < F; ++f)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) to[f][i] = load_16_bytes(from[f][i] + st * kStep);
+    };
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d)
+      if (w + d * kWaves < whole) load(next[d], w + d * kWaves);
+    for (int st0 = w; st0 < steps; st0 += kDepth * kWaves) {
+#pragma unroll
+      for (int d = 0; d < kDepth; ++d) {
+        const int st = st0 + d * kWaves;
+        if (st >= steps) break;
+        if (ROWS == kWhole || st < whole) {
+#pragma unroll
+          for (int f = 0; f < F; ++f)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) stage[f * 128 + place8(i * 8 + r, c)] = next[d][f][i];
+          if (st + kDepth * kWaves < whole) load(next[d], st + kDepth * kWaves);
+        } else {   // (the rest of the rows)
+#pragma unroll 1
+          for (int f = 0; f < F; ++f)
+#pragma unroll 1
+            for (int i = 0; i < 2; ++i)
+              stage[f * 128 + place8(i * 8 + r, c)] = load_piece(row_of(f, i * 8 + r), st * kStep + c * kLane, K, K);
+        }
+        wave_fence();
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          Frag<T> f[F];
+#pragma unroll
+          for (int i = 0; i < F; ++i) f[i].v = __builtin_bit_cast(decltype(f[i].v), stage[i * 128 + place8(m, half * 4 + quad)]);
+          multiply(f);
+        }
+        wave_fence();
+      }
+    }
+  } else {
+    for (int st = w; st < steps; st += kWaves) {
+#pragma unroll 1
+      for (int k = st * kStep + quad * kLane; k < (st + 1) * kStep; k += 4 * kLane) {
+        Frag<T> f[F];
+#pragma unroll
+        for (int i = 0; i < F; ++i) f[i] = load_frag(row_of(i, m), k, K);
+        multiply(f);
+      }
+    }
+  }
+}
+
+// The sums of the waves' parts: done(row, column, sum) for each, spread over the block's threads.
+template <int RT, int CT, typename Done>
+__device__ __forceinline__ void sum_parts(uint4* lds, const f32x4 (&acc)[RT][CT], Done done) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  __syncthreads();   // (the rows that lay there have been used)
+  f32x4* part = (f32x4*)lds;
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) part[(w * RT * CT + rt * CT + ct) * 64 + lane] = acc[rt][ct];
+  __syncthreads();
+  for (int o = threadIdx.x; o < RT * CT * 256; o += kWaves * 64) {
+    const int f = o >> 8, l = (o >> 2) & 63;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) sum += ((const float*)lds)[i * (RT * CT * 256) + o];
+    done(f / CT * 16 + (l >> 4) * 4 + (o & 3), f % CT * 16 + (l & 15), sum);
+  }
+}
+template <int RT, int CT> constexpr int kStageRows = kWaves * (RT + CT) * 128;   // the memory of both, in 16 bytes
+template <int RT, int CT> constexpr int kStageParts = kWaves * RT * CT * 64;
+
+template <typename T> constexpr int kTerms = sizeof(T) == 2 ? 2 : 1;   // numbers whose sum is one of h
+
+// A number of h: 32 bits, or two bfloat16 numbers whose sum it is, `plane` apart (an infinite one is alone).
+__device__ __forceinline__ void store_h(float* h, int64_t at, int64_t, float sum) { h[at] = sum; }
+__device__ __forceinline__ void store_h(bf16* h, int64_t at, int64_t plane, float sum) {
+  const bf16 high = from_f32<bf16>(sum);
+  const float rest = sum - to_f32(high);
+  h[at] = high;
+  h[plane + at] = from_f32<bf16>(__builtin_isfinite(rest) ? rest : 0.f);
+}
+
 // h of 16 RT rows and 16 CT columns.
 template <typename T, int RT, int CT, Rows ROWS>
-__global__ __launch_bounds__(kShrinkWaves * 64, RT == 1 ? 4 : 2) void adapter_shrink_kernel(const AdapterArgs a, int groups, int total, int more) {
-  constexpr int F = RT + CT, kLane = Frag<T>::kLane, kStep = 8 * kLane;   // (a step: 128 bytes of each row, two products)
-  constexpr int kDepth = RT == 1 && ROWS == kWhole ? 3 : 2;   // steps on their way
-  constexpr int kStage = kShrinkWaves * F * 128, kPart = kShrinkWaves * RT * CT * 64;
-  __shared__ uint4 lds[kStage > kPart ? kStage : kPart];
+__global__ __launch_bounds__(kWaves * 64, RT == 1 ? 4 : 2) void adapter_shrink_kernel(const AdapterArgs a, int groups, int total, int more) {
+  __shared__ uint4 lds[std::max(kStageRows<RT, CT>, kStageParts<RT, CT>)];
   // `more` > 0: tiles have a block for their first adapters only, and as many more look for the further ones; else as in the other
   // kernel every gridDim.y'th.
   int further = RT > 1 ? (int)blockIdx.x - (int)(gridDim.x - more) : -1, tile_at = 0, group = 0, pass = blockIdx.y;
   if (further < 0 && !place_of(blockIdx.x, RT > 1, groups, total, tile_at, group)) return;
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quad = lane >> 4, m = lane & 15, C = a.S * a.R;
-  const int steps = (a.K + kStep - 1) / kStep;
+  const int m = threadIdx.x & 15, C = a.S * a.R;
   for (bool once = false;; once = true) {
     if (once) {
       if (RT > 1 && more && further < 0) return;
@@ -224,135 +340,42 @@ __global__ __launch_bounds__(kShrinkWaves * 64, RT == 1 ? 4 : 2) void adapter_sh
       __syncthreads();   // (the memory is the next products')
     }
     if (RT > 1 && further >= 0) {
-      pass = find_further<kShrinkWaves>(a, further / groups, (int*)lds, tile_at);
+      pass = find_further<kWaves>(a, further / groups, (int*)lds, tile_at);
       if (pass < 0) return;
       group = further % groups;
       further += more;
       __syncthreads();
     }
     const int t0 = tile_at * (16 * RT), j0 = group * (CT * 16);
-    TileAdapters<RT> tile(a, t0);
     unsigned long long rows;
-    int rank, g = -1;
-    for (int i = 0; tile.left && i <= pass; ++i) {
-      const int next = tile.next(a, rows, rank);
-      if (i == pass) g = next;
-    }
+    int rank;
+    const int g = TileAdapters<RT>(a, t0).at(a, pass, rows, rank);
     if (g < 0) return;
     bool any = false;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) any |= j0 + ct * 16 + m < C && (j0 + ct * 16 + m) % a.R < rank;
     if (!__ballot(any)) continue;
-    // row `r` of the 16 F that meet here: x's, then A's
-    auto row_of = [&](int f, int r) -> const T* {
+    f32x4 acc[RT][CT];
+    products<T, RT, CT, ROWS>(a.K, lds, acc, [&](int f, int r) -> const T* {
       if (f < RT) return (const T*)a.x + (int64_t)min(t0 + f * 16 + r, a.T - 1) * a.ldx;
       return (const T*)a.a + ((int64_t)g * C + min(j0 + (f - RT) * 16 + r, C - 1)) * a.K;
-    };
-    f32x4 acc[RT][CT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) acc[rt][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto multiply = [&](const Frag<T> (&f)[F]) {
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) acc[rt][ct] = Frag<T>::mma(f[rt], f[RT + ct], acc[rt][ct]);
-    };
-    // wave w takes the steps w, w + 8, ..
-    if constexpr (ROWS != kSingle) {
-      uint4* stage = lds + w * (F * 128);
-      const int r = lane >> 3, c = lane & 7, whole = a.K / kStep;
-      const T* from[F][2];
-      uint4 next[kDepth][F][2];
-#pragma unroll
-      for (int f = 0; f < F; ++f)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) from[f][i] = row_of(f, i * 8 + r) + c * kLane;
-      auto load = [&](uint4 (&to)[F][2], int st) {
-#pragma unroll
-        for (int f = 0; f < F; ++f)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) to[f][i] = load_16_bytes(from[f][i] + st * kStep);
-      };
-#pragma unroll
-      for (int d = 0; d < kDepth; ++d)
-        if (w + d * kShrinkWaves < whole) load(next[d], w + d * kShrinkWaves);
-      for (int st0 = w; st0 < steps; st0 += kDepth * kShrinkWaves) {
-#pragma unroll
-        for (int d = 0; d < kDepth; ++d) {
-          const int st = st0 + d * kShrinkWaves;
-          if (st >= steps) break;
-          if (ROWS == kWhole || st < whole) {
-#pragma unroll
-            for (int f = 0; f < F; ++f)
-#pragma unroll
-              for (int i = 0; i < 2; ++i) stage[f * 128 + place8(i * 8 + r, c)] = next[d][f][i];
-            if (st + kDepth * kShrinkWaves < whole) load(next[d], st + kDepth * kShrinkWaves);
-          } else {   // (the rest of the rows)
-#pragma unroll 1
-            for (int f = 0; f < F; ++f)
-#pragma unroll 1
-              for (int i = 0; i < 2; ++i)
-                stage[f * 128 + place8(i * 8 + r, c)] = load_piece(row_of(f, i * 8 + r), st * kStep + c * kLane, a.K, a.K);
-          }
-          wave_fence();
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            Frag<T> f[F];
-#pragma unroll
-            for (int i = 0; i < F; ++i) f[i].v = __builtin_bit_cast(decltype(f[i].v), stage[i * 128 + place8(m, half * 4 + quad)]);
-            multiply(f);
-          }
-          wave_fence();
-        }
-      }
-    } else {
-      for (int st = w; st < steps; st += kShrinkWaves) {
-#pragma unroll 1
-        for (int k = st * kStep + quad * kLane; k < (st + 1) * kStep; k += 4 * kLane) {
-          Frag<T> f[F];
-#pragma unroll
-          for (int i = 0; i < F; ++i) f[i] = load_frag(row_of(i, m), k, a.K);
-          multiply(f);
-        }
-      }
-    }
-    __syncthreads();
-    f32x4* part = (f32x4*)lds;
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) part[(w * RT * CT + rt * CT + ct) * 64 + lane] = acc[rt][ct];
-    __syncthreads();
-    for (int o = threadIdx.x; o < RT * CT * 256; o += kShrinkWaves * 64) {
-      const int f = o >> 8, l = (o >> 2) & 63, row = f / CT * 16 + (l >> 4) * 4 + (o & 3), j = j0 + f % CT * 16 + (l & 15);
-      float sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < kShrinkWaves; ++i) sum += ((const float*)lds)[i * (RT * CT * 256) + o];
-      if (!(rows >> row & 1) || j >= C || j % a.R >= rank) continue;
-      const int64_t at = (int64_t)(t0 + row) * C + j;
-      if constexpr (sizeof(T) == 4) {
-        ((float*)a.h)[at] = sum;
-      } else {   // two numbers whose sum it is; an infinite one is alone
-        const bf16 high = from_f32<bf16>(sum);
-        const float rest = sum - to_f32(high);
-        ((bf16*)a.h)[at] = high;
-        ((bf16*)a.h)[(int64_t)a.T * C + at] = from_f32<bf16>(__builtin_isfinite(rest) ? rest : 0.f);
-      }
-    }
+    });
+    sum_parts(lds, acc, [&](int row, int col, float sum) {
+      const int j = j0 + col;
+      if (rows >> row & 1 && j < C && j % a.R < rank) store_h((T*)a.h, (int64_t)(t0 + row) * C + j, (int64_t)a.T * C, sum);
+    });
   }
 }
 
 constexpr int kRow = 68;   // floats of a row of 64 in a wave's memory: so padded that rows' columns lie in different banks
-template <typename T> constexpr int kTerms = sizeof(T) == 2 ? 2 : 1;   // numbers whose sum is one of h
 
 // 16 RT rows from t0 on and the `set`th 64 columns, by one wave: what the tile's `pass`th adapter adds to its rows; with `copy` the
-// rows without an adapter too. False: the tile has no such adapter.
+// rows without an adapter too. h: all slices' numbers of row 0, rows `hstride` apart. False: the tile has no such adapter.
 template <typename T, int RT, bool VEC>
-__device__ __forceinline__ bool expand_tile(const AdapterArgs& a, int t0, int set, int sets, int pass, bool copy, uint4* stage, bool vec_out) {
+__device__ __forceinline__ bool expand_tile(const AdapterArgs& a, const T* h, int hstride, int64_t plane, int t0, int set, int sets, int pass,
+                                            bool copy, uint4* stage, bool vec_out) {
   constexpr int kLane = Frag<T>::kLane, kStep = 4 * kLane;   // (a step: 64 bytes of each row, one product; two for h's two numbers)
-  const int lane = threadIdx.x & 63, quad = lane >> 4, m = lane & 15, C = a.S * a.R;
+  const int lane = threadIdx.x & 63, quad = lane >> 4, m = lane & 15;
   if (set >= sets) return false;
   int s = 0;
   for (; s < a.S - 1; ++s) {
@@ -363,8 +386,7 @@ __device__ __forceinline__ bool expand_tile(const AdapterArgs& a, int t0, int se
   const int c0 = a.first[s] + set * 64, end = a.first[s + 1], n = min(end - c0, 64);
   const T* base = (const T*)a.base + c0;
   T* out = (T*)a.out + c0;
-  const T* h = (const T*)a.h + s * a.R;
-  const int64_t plane = (int64_t)a.T * C;
+  h += s * a.R;
 
   // Rows as they lie in memory: 16 bytes a lane, kCols of them side by side.
   constexpr int kEach = 16 / sizeof(T), kCols = 64 / kEach, kRows = 64 / kCols;
@@ -415,17 +437,14 @@ __device__ __forceinline__ bool expand_tile(const AdapterArgs& a, int t0, int se
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) store(rt, here & ~tile.left, 0.f, nullptr);
   }
-  unsigned long long rows = 0;
-  int rank = 0, g = -1;
-  for (int i = 0; tile.left && i <= pass; ++i) {
-    const int next = tile.next(a, rows, rank);
-    if (i == pass) g = next;
-  }
+  unsigned long long rows;
+  int rank;
+  const int g = tile.at(a, pass, rows, rank);
   if (g < 0) return false;
   const float scale = a.scale[g];
   if (pass) load_base(rows);
   auto brow = [&](int j, int r) { return (const T*)a.b + ((int64_t)g * a.N + min(c0 + j * 16 + r, end - 1)) * a.R; };
-  auto hrow = [&](int rt, int r) { return h + (int64_t)min(t0 + rt * 16 + r, a.T - 1) * C; };
+  auto hrow = [&](int rt, int r) { return h + (int64_t)min(t0 + rt * 16 + r, a.T - 1) * hstride; };
   f32x4 acc[RT][4];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt)
@@ -492,12 +511,13 @@ __device__ __forceinline__ bool expand_tile(const AdapterArgs& a, int t0, int se
   return true;
 }
 
+template <typename T, int RT> constexpr int kStageExpand = std::max((4 + RT * kTerms<T>) * 64, 16 * kRow / 4);   // a wave's, in 16 bytes
+
 // Four waves take neighbouring columns. `more`: as in the other kernel.
 template <typename T, int RT, bool VEC>
 __global__ __launch_bounds__(kExpandWaves * 64, RT == 1 ? 4 : 3) void adapter_expand_kernel(const AdapterArgs a, int sets, int groups, int total, int more,
                                                                            bool vec_out) {
-  constexpr int kStage = (4 + RT * kTerms<T>) * 64, kTile = 16 * kRow / 4;
-  __shared__ uint4 lds[kExpandWaves][kStage > kTile ? kStage : kTile];
+  __shared__ uint4 lds[kExpandWaves][kStageExpand<T, RT>];
   __shared__ int counts[64];
   int further = RT > 1 && (int)blockIdx.x < more ? (int)blockIdx.x : -1, tile = 0, group = 0, pass = blockIdx.y;
   if (further < 0 && !place_of(blockIdx.x - more, RT > 1, groups, total, tile, group)) return;
@@ -509,9 +529,54 @@ __global__ __launch_bounds__(kExpandWaves * 64, RT == 1 ? 4 : 3) void adapter_ex
       group = further % groups;
       further += more;
     }
-    const bool had = expand_tile<T, RT, VEC>(a, tile * (16 * RT), group * kExpandWaves + wave, sets, pass, pass == 0 && a.base != a.out,
+    const bool had = expand_tile<T, RT, VEC>(a, (const T*)a.h, a.S * a.R, (int64_t)a.T * a.S * a.R, tile * (16 * RT), group * kExpandWaves + wave, sets, pass, pass == 0 && a.base != a.out,
                                              lds[wave], vec_out);
     if (further < 0 && (more || !had)) return;
+  }
+}
+
+// Up to 16 rows and ranks up to kFewRank in one launch: a block makes the h that its columns (512 of a slice) need itself, into its
+// own memory, in the order of the other kernels' sums. The factor A is read by every block of its slice, out of L2; what this saves
+// is a launch and the wait for the first one's end. us in one and in two launches, rows of 2,048 numbers, adapters of their own: rank
+// 16, 2,048 columns, one row 6.8 and 8.4; 3 x 2,048, 8 rows 10.0 and 10.9. With larger ranks every block has too much to read: rank
+// 64, 3 x 2,048 columns, one row 10.4 and 9.1, 16 rows 14.1 and 11.5.
+constexpr int kFewRows = 16, kFewRank = 16;
+
+template <typename T, Rows ROWS, bool VEC>
+__global__ __launch_bounds__(kWaves * 64, 2) void adapter_few_kernel(const AdapterArgs a, int sets, bool vec_out) {
+  __shared__ uint4 lds[std::max(std::max(kStageRows<1, 1>, kStageParts<1, 1>), kWaves * kStageExpand<T, 1>)];
+  __shared__ uint4 h_lds[kFewRows * kFewRank * 4 / 16];
+  int s = 0, first_set = 0, block = blockIdx.x, here = 0;
+  for (;; ++s) {
+    here = (a.first[s + 1] - a.first[s] + 63) / 64;
+    const int blocks = (here + kWaves - 1) / kWaves;
+    if (block < blocks) break;
+    block -= blocks;
+    first_set += here;
+  }
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), local = block * kWaves + wave;
+  const int stride = (a.R + 7) / 8 * 8;   // (pieces of 16 bytes begin at multiples of 16)
+  const int64_t plane = (int64_t)kFewRows * stride;
+  T* h = (T*)h_lds;
+  for (int pass = blockIdx.y;; pass += gridDim.y) {
+    unsigned long long rows;
+    int rank;
+    const int g = TileAdapters<1>(a, 0).at(a, pass, rows, rank);
+    if (g >= 0 && rank > 0) {
+      f32x4 acc[1][1];
+      products<T, 1, 1, ROWS>(a.K, lds, acc, [&](int f, int r) -> const T* {
+        if (f == 0) return (const T*)a.x + (int64_t)min(r, a.T - 1) * a.ldx;
+        return (const T*)a.a + ((int64_t)g * a.S * a.R + s * a.R + min(r, a.R - 1)) * a.K;
+      });
+      sum_parts(lds, acc, [&](int row, int col, float sum) {
+        if (col < rank) store_h(h, row * stride + col, plane, sum);
+      });
+      __syncthreads();
+    }
+    expand_tile<T, 1, VEC>(a, h - s * a.R, stride, plane, 0, local < here ? first_set + local : sets, sets, pass,
+                           pass == 0 && a.base != a.out, lds + wave * kStageExpand<T, 1>, vec_out);
+    if (g < 0) return;
+    __syncthreads();   // (both memories are the next pass's)
   }
 }
 
@@ -525,31 +590,53 @@ static dim3 grid_of(const AdapterArgs& a, int total, int* more) {
   return dim3((total + kXcds - 1) / kXcds * kXcds + *more);
 }
 
+// How a call's rows can be read and written.
+template <typename T>
+struct Forms {
+  bool x, b, out;   // 16 bytes at a time: x and A, B, base and out
+  bool rest;        // x and A: with a rest behind the whole steps
+  int sets;         // 64 columns each, of all slices
+  explicit Forms(const AdapterArgs& a) {
+    auto four = [](const void* p, long long stride) { return (uintptr_t)p % 4 == 0 && stride * sizeof(T) % 4 == 0; };
+    x = four(a.x, a.ldx) && four(a.a, a.K);
+    rest = a.K % (8 * Frag<T>::kLane) != 0;
+    b = four(a.b, a.R);
+    out = four(a.base, a.ldb) && four(a.out, a.ldo);
+    sets = 0;
+    for (int s = 0; s < a.S; ++s) {
+      sets += (a.first[s + 1] - a.first[s] + 63) / 64;
+      out &= a.first[s] * sizeof(T) % 4 == 0;
+    }
+  }
+};
+
 template <typename T, int RT, int CT>
-static void shrink(const AdapterArgs& a, hipStream_t stream) {
+static void shrink(const AdapterArgs& a, const Forms<T>& f, hipStream_t stream) {
   const int groups = (a.S * a.R + CT * 16 - 1) / (CT * 16), total = (a.T + 16 * RT - 1) / (16 * RT) * groups;
   int more = 0;
   const dim3 grid = grid_of<RT>(a, total, &more);
-  const bool vec = (uintptr_t)a.x % 4 == 0 && (uintptr_t)a.a % 4 == 0 && a.K * sizeof(T) % 4 == 0 && a.ldx * sizeof(T) % 4 == 0;
-  if (!vec) adapter_shrink_kernel<T, RT, CT, kSingle><<<grid, kShrinkWaves * 64, 0, stream>>>(a, groups, total, more);
-  else if (a.K % (8 * Frag<T>::kLane)) adapter_shrink_kernel<T, RT, CT, kRest><<<grid, kShrinkWaves * 64, 0, stream>>>(a, groups, total, more);
-  else adapter_shrink_kernel<T, RT, CT, kWhole><<<grid, kShrinkWaves * 64, 0, stream>>>(a, groups, total, more);
+  if (!f.x) adapter_shrink_kernel<T, RT, CT, kSingle><<<grid, kWaves * 64, 0, stream>>>(a, groups, total, more);
+  else if (f.rest) adapter_shrink_kernel<T, RT, CT, kRest><<<grid, kWaves * 64, 0, stream>>>(a, groups, total, more);
+  else adapter_shrink_kernel<T, RT, CT, kWhole><<<grid, kWaves * 64, 0, stream>>>(a, groups, total, more);
 }
 
 template <typename T, int RT>
-static void expand(const AdapterArgs& a, hipStream_t stream) {
-  int sets = 0;
-  bool vec_out = (uintptr_t)a.out % 4 == 0 && (uintptr_t)a.base % 4 == 0 && a.ldo * sizeof(T) % 4 == 0 && a.ldb * sizeof(T) % 4 == 0;
-  for (int s = 0; s < a.S; ++s) {
-    sets += (a.first[s + 1] - a.first[s] + 63) / 64;
-    vec_out &= a.first[s] * sizeof(T) % 4 == 0;
-  }
-  const int groups = (sets + kExpandWaves - 1) / kExpandWaves, total = (a.T + 16 * RT - 1) / (16 * RT) * groups;
+static void expand(const AdapterArgs& a, const Forms<T>& f, hipStream_t stream) {
+  const int groups = (f.sets + kExpandWaves - 1) / kExpandWaves, total = (a.T + 16 * RT - 1) / (16 * RT) * groups;
   int more = 0;
   const dim3 grid = grid_of<RT>(a, total, &more);
-  const bool vec = (uintptr_t)a.b % 4 == 0 && a.R * sizeof(T) % 4 == 0;
-  if (vec) adapter_expand_kernel<T, RT, true><<<grid, kExpandWaves * 64, 0, stream>>>(a, sets, groups, total, more, vec_out);
-  else adapter_expand_kernel<T, RT, false><<<grid, kExpandWaves * 64, 0, stream>>>(a, sets, groups, total, more, vec_out);
+  if (f.b) adapter_expand_kernel<T, RT, true><<<grid, kExpandWaves * 64, 0, stream>>>(a, f.sets, groups, total, more, f.out);
+  else adapter_expand_kernel<T, RT, false><<<grid, kExpandWaves * 64, 0, stream>>>(a, f.sets, groups, total, more, f.out);
+}
+
+template <typename T>
+static void few(const AdapterArgs& a, const Forms<T>& f, hipStream_t stream) {
+  int blocks = 0;
+  for (int s = 0; s < a.S; ++s) blocks += ((a.first[s + 1] - a.first[s] + 63) / 64 + kWaves - 1) / kWaves;
+  const dim3 grid(blocks, std::min(a.T, a.L));
+  if (!f.x || !f.b) adapter_few_kernel<T, kSingle, false><<<grid, kWaves * 64, 0, stream>>>(a, f.sets, f.out);
+  else if (f.rest) adapter_few_kernel<T, kRest, true><<<grid, kWaves * 64, 0, stream>>>(a, f.sets, f.out);
+  else adapter_few_kernel<T, kWhole, true><<<grid, kWaves * 64, 0, stream>>>(a, f.sets, f.out);
 }
 
 // Blocks of 32 rows and 64 columns of the first product from which these are the faster ones: blocks of 16 by 16 are many more. us so
@@ -560,13 +647,16 @@ template <typename T> constexpr int kManyBlocks = sizeof(T) == 2 ? 48 : 192;
 
 template <typename T>
 static void launch(const AdapterArgs& a, hipStream_t stream) {
+  const Forms<T> f(a);
   const long long blocks = (a.T + 31ll) / 32 * ((a.S * a.R + 63) / 64);
-  if (blocks >= kManyBlocks<T> && !a.single) {
-    shrink<T, 2, 4>(a, stream);
-    expand<T, 2>(a, stream);
+  if (a.T <= kFewRows && a.R <= kFewRank) {
+    few(a, f, stream);
+  } else if (blocks >= kManyBlocks<T> && !a.single) {
+    shrink<T, 2, 4>(a, f, stream);
+    expand<T, 2>(a, f, stream);
   } else {
-    shrink<T, 1, 1>(a, stream);
-    expand<T, 1>(a, stream);
+    shrink<T, 1, 1>(a, f, stream);
+    expand<T, 1>(a, f, stream);
   }
 }
 
@@ -574,6 +664,9 @@ static void launch(const AdapterArgs& a, hipStream_t stream) {
 
 using namespace ninfer;
 
+// Rows and ranks up to which a call needs no scratch.
+extern "C" int ninfer_adapter_few_rows() { return kFewRows; }
+extern "C" int ninfer_adapter_few_rank() { return kFewRank; }
 extern "C" int ninfer_adapter_args_bytes() { return (int)sizeof(AdapterArgs); }
 
 extern "C" int ninfer_adapter_add(const AdapterArgs* args, hipStream_t stream) {
@@ -583,7 +676,8 @@ extern "C" int ninfer_adapter_add(const AdapterArgs* args, hipStream_t stream) {
   NINFER_REQUIRE(a.S >= 1 && a.S <= 4 && a.first[0] == 0 && a.first[a.S] == a.N, "adapter_add: %d slices of %d columns", a.S, a.N);
   for (int s = 0; s < a.S; ++s)
     NINFER_REQUIRE(a.first[s] < a.first[s + 1], "adapter_add: slice %d has no columns", s);
-  NINFER_REQUIRE(a.x && a.a && a.b && a.scale && a.ranks && a.row_adapter && a.base && a.out && a.h, "adapter_add: a required array is null");
+  NINFER_REQUIRE(a.x && a.a && a.b && a.scale && a.ranks && a.row_adapter && a.base && a.out && (a.h || (a.T <= kFewRows && a.R <= kFewRank)),
+                 "adapter_add: a required array is null");
   NINFER_REQUIRE(a.ldx >= a.K && a.ldb >= a.N && a.ldo >= a.N, "adapter_add: a row stride is less than the row");
   NINFER_REQUIRE(a.base != a.out || a.ldb == a.ldo, "adapter_add: in place with two row strides");
   // (threads of a grid's x, in blocks of 16 rows: 512 for 16 columns of h, 64 for 64 of out)

@@ -381,6 +381,9 @@ class HipOps:
                            (_LOGPROB_ARGS, self.lib.ninfer_logprob_args_bytes)):
             if size() != args.size:
                 raise KernelError(f"{self.lib_path} and these bindings lay arguments out differently ({args.format})")
+        if (self.lib.ninfer_adapter_few_rows(), self.lib.ninfer_adapter_few_rank(), self.lib.ninfer_logprob_most()) != (
+                self.ADAPTER_FEW_ROWS, self.ADAPTER_FEW_RANK, self.LISTED_TOKENS):
+            raise KernelError(f"{self.lib_path} and these bindings differ on what few rows and the most listed tokens are")
         self.lib.ninfer_logprob_scratch_bytes.restype = ctypes.c_longlong
         self.lib.ninfer_attention_workspace_floats.restype = ctypes.c_longlong
         self.lib.ninfer_event_create.restype = ctypes.c_void_p
@@ -2252,6 +2255,8 @@ class HipOps:
     def _stream_of(device: int) -> int:
         return torch.cuda.current_stream(device).cuda_stream if _raw_stream is None else _raw_stream(device)
 
+    ADAPTER_FEW_ROWS, ADAPTER_FEW_RANK = 16, 16   # the library's own
+
     def adapter_add(self, x, a, b, scale, ranks, widths, row_adapter, out, base=None, single_rows=0):
         """Low-rank adapters of many requests beside a projection whose output `base` [T, N] is (None: `out`, in place): for
         row t with adapter g = row_adapter[t] and every slice s of the columns (`widths`: their sizes, up to four),
@@ -2295,12 +2300,14 @@ class HipOps:
         if (pb != po or ldb != ldo) and pb < end_o and po < end_b:
             raise KernelError("adapter_add: base and out overlap")
         self._here(dev)
-        h = torch.empty(t * slices * r, dtype=torch.float32, device=x.device)
+        h = None   # (few rows need no scratch)
+        if t > self.ADAPTER_FEW_ROWS or r > self.ADAPTER_FEW_RANK:
+            h = torch.empty(t * slices * r, dtype=torch.float32, device=x.device)
         first = [0, n, n, n, n]
         for i in range(1, slices):
             first[i] = first[i - 1] + widths[i - 1]
         lib, stream, code = self.lib, self._stream_of(dev), _DT[dt]
-        pa, p_b, ph = a.data_ptr(), b.data_ptr(), h.data_ptr()
+        pa, p_b, ph = a.data_ptr(), b.data_ptr(), 0 if h is None else h.data_ptr()
         # (single rows beside others: tiles of their own, where there are enough rows for two forms)
         for lo, hi in ((0, single_rows), (single_rows, t)) if 0 < single_rows < t and t >= 512 else ((0, t),):
             args = _ADAPTER_ARGS.pack(px + lo * ldx * size, pa, p_b, p_scale, p_ranks, p_rows + 4 * lo, pb + lo * ldb * size,

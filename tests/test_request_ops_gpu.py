@@ -51,7 +51,7 @@ def rows_of(kind, t, count, rng):
 @pytest.mark.parametrize("t,k,widths,r,count", [
     (1, 64, (64,), 16, 1), (1, 2048, (256, 64, 64), 16, 4), (2, 1, (1,), 1, 2), (3, 33, (7, 5, 1, 2), 3, 3),
     (15, 96, (48,), 8, 5), (16, 128, (64, 32, 32), 32, 16), (17, 1000, (100, 60), 24, 7), (64, 512, (192, 64), 64, 8),
-    (65, 257, (65, 63, 64), 20, 3), (130, 320, (130,), 40, 2), (700, 264, (72, 8, 16), 12, 6), (33, 72, (16,), 129, 4)])
+    (65, 257, (65, 63, 64), 20, 3), (130, 320, (130,), 40, 2), (700, 264, (72, 8, 16), 12, 6), (33, 72, (16,), 129, 4), (9, 72, (16, 600), 100, 4), (16, 2048, (1100, 70), 64, 16), (16, 2048, (1100, 70), 16, 16), (11, 1030, (513, 9, 30, 64), 13, 40)])
 @pytest.mark.parametrize("kind", ["one", "mixed", "portions"])
 def test_adapters(ops, dtype, t, k, widths, r, count, kind):
     rng = random.Random(t * 7 + k)
@@ -148,6 +148,20 @@ def test_adapters_give_a_row_the_same_bits_in_any_company(ops):
     out = torch.empty_like(base)
     ops.adapter_add(x, a, b, scale, ranks, widths, i32(rows), out, base=base)
     for some in ([0], [5], list(range(100, 116)), list(range(3, 640, 11)), list(range(128, 400))):
+        got = torch.empty_like(base[some])
+        ops.adapter_add(x[some], a, b, scale, ranks, widths, i32([rows[i] for i in some]), got, base=base[some])
+        assert torch.equal(got, out[some])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_adapters_of_small_rank_give_a_row_the_same_bits_in_any_company(ops, dtype):
+    # (16 rows go through one launch, more through two)
+    t, k, widths, r, count = 50, 1000, (600, 64), 16, 6
+    x, a, b, scale, base = tables(count, k, widths, r, dtype, 10, t)
+    ranks, rows = i32([16, 3, 16, 0, 9, 16]), [i * 5 % 7 - 1 for i in range(t)]
+    out = torch.empty_like(base)
+    ops.adapter_add(x, a, b, scale, ranks, widths, i32(rows), out, base=base)
+    for some in ([0], [5], list(range(16)), list(range(30, 39)), list(range(3, 50, 4))):
         got = torch.empty_like(base[some])
         ops.adapter_add(x[some], a, b, scale, ranks, widths, i32([rows[i] for i in some]), got, base=base[some])
         assert torch.equal(got, out[some])

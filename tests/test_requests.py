@@ -421,7 +421,7 @@ def test_the_library_refuses(lib):
         return args.pack(*[x for v in values for x in (v if isinstance(v, list) else [v or 0])])
 
     first = [0, 64, 96, 0, 0]
-    fine = dict(x=p, a=p, b=p, scale=p, ranks=p, row_adapter=p, base=p, out=p, h=p, ldx=64, ldb=96, ldo=96, T=4, K=64, R=8, S=2, L=2, N=96,
+    fine = dict(x=p, a=p, b=p, scale=p, ranks=p, row_adapter=p, base=p, out=p, h=p, ldx=64, ldb=96, ldo=96, T=17, K=64, R=8, S=2, L=2, N=96,
                 first=first, dtype=1)
     for change, match in ((dict(T=0), "positive"), (dict(K=0), "positive"), (dict(R=-1), "positive"), (dict(L=0), "positive"), (dict(S=0), "slices"),
                           (dict(S=5), "slices"), (dict(N=95), "slices"), (dict(first=[0, 96, 96, 0, 0]), "no columns"),
