@@ -37,7 +37,7 @@ constexpr int kAdjustLists = 8;   // list entries a thread has on their way at a
 
 // l / p^count, or l p^count for a logit that is not positive: the power by squaring, at most 31 turns.
 __device__ __forceinline__ float penalised(float l, float p, unsigned count) {
-  if (l == 0.f) return l;   // (p^count may be infinite)
+  if (l == 0.f || fabsf(l) == INFINITY) return l;   // (p^count may be infinite, or 0)
   double power = 1., square = p;
   for (; count; count >>= 1, square *= square)
     if (count & 1) power *= square;

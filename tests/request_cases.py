@@ -49,7 +49,7 @@ def adjusted(logits, repetition=None, presence=None, frequency=None, histories=N
                 continue
             x = float(v[r, token])
             p = float(repetition[r]) if repetition is not None else 1.0
-            if p != 1.0 and x != 0 and c:
+            if p != 1.0 and x != 0 and not math.isinf(x) and c:
                 try:
                     power = p ** c
                 except OverflowError:

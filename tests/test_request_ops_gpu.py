@@ -297,8 +297,8 @@ def test_adjust_rows_of_wider_ones(ops, shift, pad):
 
 
 def test_adjust_counts_of_any_size(ops):
-    logits = f32([[2.0, -2.0, 0.0, 1e30, -1e30, 3.0]])
-    counts = [2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 1, 300, 300, 70000]
+    logits = f32([[2.0, -2.0, 0.0, 1e30, -1e30, 3.0, INF, -INF]])
+    counts = [2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 1, 300, 300, 70000, 90000, 90000]
     for p in (1.5, 0.5, 1.0 + 2.0 ** -23, 1.0000001192092896):
         c = dict(repetition=[p], presence=[0.5], frequency=[0.0], histories=[[(t, n, 0) for t, n in enumerate(counts)]],
                  biases=None, masks=None, mask_rows=None)
