@@ -280,6 +280,8 @@ class Ninfer:
         for prompt, adapter in zip(prompts, adapters):
             if len(prompt) == 0:
                 raise ValueError("a prompt to score needs at least one token")
+            if not 0 <= min(prompt) <= max(prompt) < self.vocab:   # (the last token is in no step)
+                raise ValueError(f"token id outside [0, {self.vocab})")
             told: List[TokenLogprob] = []
             with self.session(adapter) as s:
                 for i in range(0, len(prompt) - 1, self.options.prefill_chunk):

@@ -387,6 +387,9 @@ def test_scores_of_prompts(tiny, tmp_path):
             eng.score([[1, 2]], **bad)
     with pytest.raises(ValueError):
         eng.score([[]])
+    for prompt in ([1, 256], [1, -1], [1 << 40], [256, 1]):
+        with pytest.raises(ValueError, match="outside"):
+            eng.score([prompt])
     eng.remove_adapter("all")
 
 
