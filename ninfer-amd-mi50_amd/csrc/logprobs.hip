@@ -14,7 +14,8 @@
 // in a fixed order and finds the best tokens from those keys: the top-th largest of 64 groups' maxima
 // is a bound that at least `top` logits reach, and only the logits of threads whose key reaches it (about
 // as many as `top`) are looked at again. A row in which very many logits are equal to the bound goes through its logits
-// once per token instead.
+// once per token instead. 512 rows of 151,936 tokens, no list: 53 us (5.9 TB/s with the join; the first launch alone 48); 64 rows with
+// their 20 best tokens 17 (10 and 7), one row 10: the second launch's waits, and the launch itself, are most of it.
 #include "sampling.h"
 #include <type_traits>
 

@@ -435,7 +435,8 @@ def test_the_library_refuses(lib):
     refuses(lib, lambda: lib.ninfer_adapter_add(None, None), "no arguments")
     fine = dict(logits=p, out=p, ld=100, ldo=100, R=2, V=100)
     for change, match in ((dict(R=0), "positive"), (dict(V=-1), "positive"), (dict(logits=None), "null"), (dict(ld=99), "stride"), (dict(ldo=104), "two row strides"),
-                          (dict(n_hist=-1), "negative"), (dict(hist_offsets=p, n_hist=3), "history"), (dict(bias_offsets=p, n_bias=3), "biases"),
+                          (dict(n_hist=-1), "negative"), (dict(n_hist=2 ** 31 - 8192), "entries are too many"),
+                          (dict(n_bias=2 ** 31 - 1), "entries are too many"), (dict(hist_offsets=p, n_hist=3), "history"), (dict(bias_offsets=p, n_bias=3), "biases"),
                           (dict(mask_rows=p, n_masks=1), "masks"), (dict(R=2 ** 31 - 1, V=100000, ld=100000, ldo=100000), "too many")):
         refuses(lib, lambda: lib.ninfer_adjust_logits(fill(_ADJUST_ARGS, **dict(fine, **change)), None), match)
     refuses(lib, lambda: lib.ninfer_adjust_logits(None, None), "no arguments")
