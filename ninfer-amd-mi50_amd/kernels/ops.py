@@ -2398,6 +2398,9 @@ class HipOps:
             args = _LOGPROB_ARGS.pack(logits.data_ptr(), pt, pl, pbf, best.data_ptr(), best_logprob.data_ptr(), 0, 0, 0, ld, r, v, top, 0)
             if self.lib.ninfer_token_logprobs(args, scratch.data_ptr(), self._stream_of(dev)):
                 self._ok(-1)
+        elif tokens is not None:
+            logprob.fill_(float("nan"))
+            before.fill_(-1)
         return logprob, before, best, best_logprob
 
     # ---- sampling -------------------------------------------------------------------

@@ -465,6 +465,16 @@ def test_rows_of_logits_beyond_32_bits(ops):
     rc.close(rows, want, room)
 
 
+def test_no_rows_and_no_tokens(ops):
+    none = torch.zeros(0, 100, device="cuda")
+    p, before, best, best_p = ops.token_logprobs(none, i32([]), 3)
+    assert p.shape == before.shape == (0,) and best.shape == best_p.shape == (0, 3)
+    ops.adjust_logits(none)
+    p, before, best, best_p = ops.token_logprobs(torch.zeros(2, 0, device="cuda"), i32([0, 5]))
+    assert p.isnan().all() and before.tolist() == [-1, -1] and best.shape == (2, 0)
+    ops.adjust_logits(torch.zeros(2, 0, device="cuda"))
+
+
 def test_logprobs_refusals(ops):
     from ninfer_amd.kernels.ops import KernelError
     x = torch.zeros(2, 50, device="cuda")
