@@ -52,6 +52,8 @@ class AdapterSet:
             raise ValueError(f"all {self.count} places for adapters are taken")
         if weights.rank > self.rank:
             raise WeightError(f"adapter {name!r} has rank {weights.rank}, there is room for {self.rank}")
+        if not abs(weights.scale) <= torch.finfo(torch.float32).max:
+            raise WeightError(f"adapter {name!r} has a scale of {weights.scale}")
         problems, known = [], {}
         for s in self.spots:
             for weight, columns in s.weights:
@@ -59,6 +61,8 @@ class AdapterSet:
         factors = {}
         for module, (a, b) in weights.factors.items():
             weight = module + ".weight" if module + ".weight" in known else module
+            if weight in factors:
+                problems.append(f"{weight} has factors twice")
             factors[weight] = (a, b)
             if weight not in known:
                 problems.append(f"{module} takes no adapter here")
@@ -80,6 +84,8 @@ class AdapterSet:
                 at += columns
             t.ranks[g] = r if here else 0
         self._scale[g] = weights.scale
+        if self._scale.is_cuda:
+            torch.cuda.synchronize(self._scale.device)   # (steps on any stream find it)
         self._names[g], self._holds[g] = name, 0
         return g
 

@@ -19,7 +19,9 @@ _NAME = re.compile(r"^(?:base_model\.model\.)?(.+)\.lora_([AB])\.weight$")
 # options under which the files mean something else, unless they have this value (or are absent)
 _PLAIN = {"use_dora": (False,), "bias": ("none",), "fan_in_fan_out": (False,), "rank_pattern": ({}, None),
           "alpha_pattern": ({}, None), "modules_to_save": ([], None), "layers_to_transform": ([], None), "lora_bias": (False,),
-          "use_qalora": (False,), "trainable_token_indices": ([], {}, None)}
+          "use_qalora": (False,), "trainable_token_indices": ([], {}, None), "peft_type": ("LORA",), "layer_replication": ([], None),
+          # (other starts change the weights beside which the factors lie, and files of such adapters may count on that)
+          "init_lora_weights": (True, False, None, "gaussian", "orthogonal", "eva")}
 
 
 @dataclass

@@ -166,6 +166,12 @@ def test_adapter_files_that_are_refused(tiny, tmp_path):
     refused("bias", bias="all")
     refused("rank_pattern", rank_pattern={"q_proj": 2})
     refused("modules_to_save", modules_to_save=["lm_head"])
+    refused("peft_type", peft_type="LOHA")
+    refused("layer_replication", layer_replication=[[0, 1]])
+    refused("init_lora_weights", init_lora_weights="pissa")
+    refused("init_lora_weights", init_lora_weights="loftq")
+    refused("scale of", alpha=1e300)
+    refused("factors twice", {name: (a, b), name[:-len(".weight")] + ".weight.weight": (a, b)})
     refused("whole number", rank=0)
     refused("whole number", rank="4")
     refused("must be a number", alpha="x")
