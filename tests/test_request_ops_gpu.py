@@ -344,6 +344,31 @@ def test_adjust_lists_of_every_token(ops, vocab):
     rc.close(logits, want, room)
 
 
+@pytest.mark.parametrize("biases", [63, 64, 65, 130])
+def test_adjust_biases_of_one_part(ops, biases):
+    rng = random.Random(biases)
+    c = dict(repetition=[1.5], presence=[0.25], frequency=[0.5], histories=[[(t, 1 + t % 3, t % 2) for t in range(0, 90, 2)]],
+             biases=[[(rng.randrange(90), rng.uniform(-4, 4)) for _ in range(biases)]], masks=None, mask_rows=None)
+    logits = torch.randn(1, 4096, generator=torch.Generator("cuda").manual_seed(biases), device="cuda")
+    want, room = rc.adjusted(logits, **rounded(c))
+    ops.adjust_logits(logits, **on_gpu(c))
+    rc.close(logits, want, room)
+
+
+@pytest.mark.parametrize("which", ["histories", "biases", "both"])
+def test_adjust_lists_of_a_million_entries(ops, which):
+    rng, n, vocab = random.Random(3), (1 << 20) + 77, 5001
+    ids = [rng.randrange(-50, vocab + 50) for _ in range(n)]
+    few = [(t, 1, 1) for t in (0, 7, 4999)], [(t, 0.5) for t in (1, 7, 4999)]
+    c = dict(repetition=[1.0 + 2.0 ** -10], presence=[0.25], frequency=[2.0 ** -9], masks=None, mask_rows=None,
+             histories=[[(t, 1, i % 2) for i, t in enumerate(ids)] if which != "biases" else few[0]],
+             biases=[[(t, (i % 64) / 8) for i, t in enumerate(ids)] if which != "histories" else few[1]])
+    logits = torch.randn(1, vocab, generator=torch.Generator("cuda").manual_seed(3), device="cuda")
+    want, room = rc.adjusted(logits, **rounded(c))
+    ops.adjust_logits(logits, **on_gpu(c))
+    rc.close(logits, want, room)
+
+
 def test_adjust_refusals(ops):
     from ninfer_amd.kernels.ops import KernelError
     logits, one = torch.zeros(2, 64, device="cuda"), f32([1.0, 1.0])
