@@ -12,8 +12,8 @@
 // adds up in shared memory what falls into its part. So the lists need no order, and a token may
 // stand in a history more than once (whole numbers: the sums are exact in every order); of several
 // biases of one token the last one of the list holds. A list is read by every block of its row, but
-// out of L2. 64 rows of 151,936 tokens with 2,500 entries each take 18.5 us (4.3 TB/s), 256 with 6,000 72 (4.6), where
-// a copy has 5.1 TB/s.
+// out of L2. 64 rows of 151,936 tokens with 2,500 entries each take 19 us (4.3 TB/s), 256 with 6,000 87 (3.9; 72 where
+// the logits lie in the memory-side cache), where a copy has 5.1 TB/s.
 #include "sampling.h"
 
 namespace ninfer {
@@ -92,7 +92,7 @@ __device__ __forceinline__ void scan_list(int (&t)[N], const int* tokens, int fi
 // What entries say is read, and the values of their tokens are made, by as many threads as there are entries in the part: in the loop over
 // the list, or over the logits that a thread holds, nearly every wave would wait for those loads, and run a power and a quotient
 // in 64 bits, in every turn (256 rows of 151,936 tokens with 6,000 entries each, us: 181 so, 141 with the values alone made so). Both lists go
-// through these steps together: a block's time is its waits, for memory and for its waves (these rows 98 one list after the other, 92 together).
+// through these steps together: a block's time is its waits, for memory and for its waves (these rows 100 one list after the other, 92 together).
 __global__ __launch_bounds__(kAdjustThreads) void adjust_logits_kernel(const AdjustArgs a, int parts) {
   __shared__ AdjustLds l;
   constexpr int kEach = ((int)kMostEntries + kAdjustThreads - 1) / kAdjustThreads;
@@ -264,7 +264,8 @@ __global__ __launch_bounds__(kAdjustThreads) void adjust_logits_kernel(const Adj
         if (!(words[u] >> ((t0 + i) & 28) >> c & 1)) v[u][c] = -INFINITY;
     }
     if (fours) {
-      // (past the L2, where the lists and the logits looked up again are: 92 us through it, 72 so; 64 rows 20.1 and 18.2)
+      // (past the L2, where the lists and the logits looked up again are: 92 us through it, 87 so, 72 with the logits in the
+      // memory-side cache; 64 rows 19.9 and 19.0)
       if (i < n) __builtin_nontemporal_store(v[u], (Four*)(to + i));
     } else {
 #pragma unroll

@@ -14,8 +14,8 @@
 // in a fixed order and finds the best tokens from those keys: the top-th largest of 64 groups' maxima
 // is a bound that at least `top` logits reach, and only the logits of threads whose key reaches it (about
 // as many as `top`) are looked at again. A row in which very many logits are equal to the bound goes through its logits
-// once per token instead. 512 rows of 151,936 tokens, no list: 51 us (6.1 TB/s with the join; the first launch alone 46); 64 rows with
-// their 20 best tokens 15 (9 and 7), one row 10: the second launch's waits, and the launch itself, are most of it.
+// once per token instead. 512 rows of 151,936 tokens, no list: 53 us (5.9 TB/s with the join; the first launch alone 48); 64 rows with
+// their 20 best tokens 17 (9 and 7), one row 10: the second launch's waits, and the launch itself, are most of it.
 #include "sampling.h"
 #include <type_traits>
 
@@ -59,8 +59,8 @@ __global__ __launch_bounds__(kLpThreads) void logprob_parts_kernel(const Logprob
   const float* row = a.logits + r * a.ld;
   const int token = a.tokens ? a.tokens[r] : -1;
   const bool asked = token >= 0 && token < a.V, whole = n == kLpPart;
-  // (as many loads whatever the part, all on their way at once, and past the L2: 64 rows of 151,936 tokens 16.2 us through it, 15.2 so;
-  // 512 rows 54 and 51)
+  // (as many loads whatever the part, all on their way at once, and past the L2: 512 rows of 151,936 tokens 58 us through it,
+  // 53 so; where the logits lie in the memory-side cache 54 and 51, 64 rows 16.2 and 15.2)
   Four v[kLpQuads];
   if (a.vec && n % 4 == 0) {
 #pragma unroll

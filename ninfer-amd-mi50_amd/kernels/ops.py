@@ -2392,7 +2392,8 @@ class HipOps:
         if tokens is not None:
             logprob, before = torch.empty(r, dtype=f32, device=device), torch.empty(r, dtype=i32, device=device)
             pl, pbf = logprob.data_ptr(), before.data_ptr()
-        best, best_logprob = torch.empty((r, top), dtype=i32, device=device), torch.empty((r, top), dtype=f32, device=device)
+        best = torch.empty_strided((r, top), (top, 1), dtype=i32, device=device)   # (a size of two numbers costs `empty` a third more)
+        best_logprob = torch.empty_strided((r, top), (top, 1), dtype=f32, device=device)
         if r and v and (top or tokens is not None):
             scratch = torch.empty(self.lib.ninfer_logprob_scratch_bytes(r, v, top), dtype=torch.uint8, device=device)
             args = _LOGPROB_ARGS.pack(logits.data_ptr(), pt, pl, pbf, best.data_ptr(), best_logprob.data_ptr(), 0, 0, 0, ld, r, v, top, 0)
