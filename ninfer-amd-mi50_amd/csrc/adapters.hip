@@ -641,25 +641,31 @@ static void few(const AdapterArgs& a, const Forms<T>& f, hipStream_t stream) {
   else adapter_few_kernel<T, kWhole, true><<<grid, kWaves * 64, 0, stream>>>(a, f.sets, f.out);
 }
 
-// Blocks of 32 rows and 64 columns of the first product from which these are the faster ones: blocks of 16 by 16 are many more. us so
-// and in blocks of 16 by 16, one adapter a tile: bfloat16, 3 x 64 columns of 2,048, 384 rows 21 and 16, 512 (48 blocks) 15.8 and 16.7,
-// 2,048 26 and 38; 64 columns, 1,024 rows (32) 14.5 and 12.8, 2,048 (64) 16 and 19; 32-bit, 3 x 64 columns, 1,024 rows (96) 48 and 43,
-// 2,048 (192) 65 and 68. Rows that each have an adapter of their own never: 512 of eight adapters in turn 95 and 69.
+// Blocks of 32 rows and 64 columns of the first product from which these are the faster ones: blocks of 16 by 16 are many more. us of both
+// products so and in blocks of 16 by 16: bfloat16, 3 x 64 columns of 2,048, 384 rows 15.7 and 13.3, 512 (48 blocks) 15.8 and 14.0, with
+// eight single rows before them 23.4 and 26.9, 1,024 rows 19.2 and 20.4, 26.5 and 39.4; 3 x 16 columns, 1,024 rows (32) 17.4 and 14.7; 32-bit,
+// 3 x 64 columns, 1,024 rows (96) 48 and 37, 2,048 (192) 64 and 64, with eight single rows 74 and 91. Rows that each have an adapter of
+// their own never: 512 of eight adapters in turn 97 and 60.
 template <typename T> constexpr int kManyBlocks = sizeof(T) == 2 ? 48 : 192;
+
+// The second product in tiles of 32 rows once these make three blocks for four CUs: as fast as in tiles of 16 where every tile has one
+// adapter, and faster by what a tile of single rows takes that has several, whose further ones are blocks of their own here and
+// one pass after the other there. us in tiles of 32 and of 16, bfloat16, 3 x 2,048 columns, rank 16, eight single rows before 256 rows of one
+// request 15.2 and 18.9, 512 16.2 and 27.8, 1,024 21 and 33, without the single rows 9.7 and 9.9, 11.0 and 11.1, 14.7 and 17.0; 32-bit,
+// rank 64, 256 rows 33 and 40, without 18.9 and 17.1.
+static bool tiles_of_32(const AdapterArgs& a, int sets) {
+  return !a.single && (a.T + 31ll) / 32 * ((sets + kExpandWaves - 1) / kExpandWaves) * 4 >= 3ll * device_cu_count();
+}
 
 template <typename T>
 static void launch(const AdapterArgs& a, hipStream_t stream) {
   const Forms<T> f(a);
   const long long blocks = (a.T + 31ll) / 32 * ((a.S * a.R + 63) / 64);
-  if (a.T <= kFewRows && a.R <= kFewRank) {
-    few(a, f, stream);
-  } else if (blocks >= kManyBlocks<T> && !a.single) {
-    shrink<T, 2, 4>(a, f, stream);
-    expand<T, 2>(a, f, stream);
-  } else {
-    shrink<T, 1, 1>(a, f, stream);
-    expand<T, 1>(a, f, stream);
-  }
+  if (a.T <= kFewRows && a.R <= kFewRank) return few(a, f, stream);
+  if (blocks >= kManyBlocks<T> && !a.single) shrink<T, 2, 4>(a, f, stream);
+  else shrink<T, 1, 1>(a, f, stream);
+  if (tiles_of_32(a, f.sets)) expand<T, 2>(a, f, stream);
+  else expand<T, 1>(a, f, stream);
 }
 
 }  // namespace ninfer

@@ -2308,8 +2308,11 @@ class HipOps:
             first[i] = first[i - 1] + widths[i - 1]
         lib, stream, code = self.lib, self._stream_of(dev), _DT[dt]
         pa, p_b, ph = a.data_ptr(), b.data_ptr(), 0 if h is None else h.data_ptr()
-        # (single rows beside others: tiles of their own, where there are enough rows for two forms)
-        for lo, hi in ((0, single_rows), (single_rows, t)) if 0 < single_rows < t and t >= 512 else ((0, t),):
+        # (Single rows of many adapters beside other rows: two calls, since a tile of theirs has an adapter a row. us so and in one call, 64
+        # adapters of rank 16 beside q, k and v of 2,048 columns: 32 of them and 512 rows 27 and 39, 2,048 rows 39 and 49; 8 of them 21 and
+        # 16, 34 and 30.)
+        apart = min(single_rows, count) >= 16 and t - single_rows >= 128
+        for lo, hi in ((0, single_rows), (single_rows, t)) if apart else ((0, t),):
             args = _ADAPTER_ARGS.pack(px + lo * ldx * size, pa, p_b, p_scale, p_ranks, p_rows + 4 * lo, pb + lo * ldb * size,
                                       po + lo * ldo * size, ph + lo * slices * r * 4, ldx, ldb, ldo, hi - lo, k, r, slices, count, n, *first, code, hi <= single_rows)
             if lib.ninfer_adapter_add(args, stream):

@@ -91,6 +91,30 @@ def test_adapters_of_many_rows(ops, dtype, t, count, kind):
     assert torch.equal(base, out)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("t,k,r,count", [(600, 136, 8, 9), (640, 129, 13, 40), (1100, 72, 64, 1), (577, 200, 80, 70)])
+@pytest.mark.parametrize("kind", ["one", "mixed", "portions", "singles"])
+def test_adapters_of_many_columns(ops, dtype, t, k, r, count, kind):
+    """Enough columns for tiles of 32 rows in the second product, whatever the first one's are."""
+    widths, rng = (1500, 77, 1000), random.Random(t)
+    x, a, b, scale, base = tables(count, k, widths, r, dtype, t, t)
+    ranks = [rng.randint(0, r) for _ in range(count)]
+    ranks[-1] = r
+    rows = [i % count for i in range(30)] + [0] * (t - 30) if kind == "singles" else rows_of(kind, t, count, rng)
+    want, room = rc.adapters(x.cpu(), a.cpu(), b.cpu(), scale.cpu(), ranks, widths, torch.tensor(rows), base.cpu())
+    out = torch.full_like(base, NAN)
+    ops.adapter_add(x, a, b, scale, i32(ranks), widths, i32(rows), out, base=base)
+    rc.close(out, want, room)
+    for single in (15, 30, t):   # (the same bits: what is said of the rows changes the time alone)
+        again = torch.full_like(base, NAN)
+        ops.adapter_add(x, a, b, scale, i32(ranks), widths, i32(rows), again, base=base, single_rows=single)
+        assert torch.equal(again, out)
+    some = list(range(0, 8)) + list(range(t - 8, t))
+    got = torch.empty_like(base[some])
+    ops.adapter_add(x[some], a, b, scale, i32(ranks), widths, i32([rows[i] for i in some]), got, base=base[some])
+    assert torch.equal(got, out[some])
+
+
 def test_adapters_rows_without_one_keep_their_bits(ops):
     x, a, b, scale, base = tables(3, 128, (64, 64), 16, torch.bfloat16, 1, 40)
     base[3, 5], base[7, 9] = NAN, INF
