@@ -5,7 +5,7 @@
 //   h[t, s, i] = sum_k A[g, s R + i, k] x[t, k]                       i < ranks[g]
 //   out[t, c] = base[t, c] + scale[g] sum_i B[g, c, i] h[t, s(c), i]
 //
-// Two launches, but for few rows of small rank: all slices' h, kept in 32 bits (scratch [T, S R]), then the columns. Both give a block
+// Two launches, but for few rows of small rank: all slices' h, with the 24 bits of its 32-bit sums (scratch [T, S R]), then the columns. Both give a block
 // tiles of 16 or 32 rows on the matrix units, whatever adapters these rows have: the products of a tile and
 // one of its adapters are a block's work, the rows of others ride along unwritten. Rows of a request are
 // neighbours, so a tile of a prompt's portion has one adapter, as a rule; a tile of single rows may have as
@@ -16,9 +16,9 @@
 // What bounds it: few rows, the latency of two launches that each wait for memory once (the factors
 // of the step's adapters are some MB: 64 rows of three slices of 2,048 numbers and eight adapters of ranks up to 64, 13 us in a
 // captured step; one row of rank 16, in one launch, 7); many rows, reading and writing x, base and out (2,055 rows of 3,584
-// numbers: 33 us, 1.9 TB/s of what cannot be spared: both launches wait for rows and factors in turn). h enters the
-// second product as a sum of two bfloat16 numbers (the rounded value and what the rounding left, 16
-// bits together), so that the only rounding of note is that of `out`.
+// numbers: 33 us, 1.9 TB/s of what cannot be spared: both launches wait for rows and factors in turn). h of bfloat16 rows enters the
+// second product as a sum of three bfloat16 numbers (the rounded value, what the rounding left, rounded, and what that left: 8 bits
+// each, 24 together), so that none of its bits is lost and `out` alone is rounded.
 //
 // A tile's sums run in the same order however many rows the step has: every form cuts k among
 // eight waves in the same way, and a request's numbers do not depend on its company.
@@ -36,7 +36,7 @@ struct AdapterArgs {
   const int* row_adapter;   // [T]; outside [0, L): none
   const void* base;      // [T, ldb]; may be out
   void* out;             // [T, ldo]
-  void* h;               // [T, S R] 32-bit numbers, or as many pairs of bfloat16 ones in two planes
+  void* h;               // [T, S R] 32-bit numbers, or as many bfloat16 ones in each of three planes (kTerms)
   long long ldx, ldb, ldo;
   int T, K, R, S, L, N;
   int first[5];          // slice s: columns first[s] .. first[s + 1]
@@ -315,15 +315,18 @@ __device__ __forceinline__ void sum_parts(uint4* lds, const f32x4 (&acc)[RT][CT]
 template <int RT, int CT> constexpr int kStageRows = kWaves * (RT + CT) * 128;   // the memory of both, in 16 bytes
 template <int RT, int CT> constexpr int kStageParts = kWaves * RT * CT * 64;
 
-template <typename T> constexpr int kTerms = sizeof(T) == 2 ? 2 : 1;   // numbers whose sum is one of h
+template <typename T> constexpr int kTerms = sizeof(T) == 2 ? 3 : 1;   // numbers whose sum is one of h
 
-// A number of h: 32 bits, or two bfloat16 numbers whose sum it is, `plane` apart (an infinite one is alone).
+// A number of h: 32 bits, or three bfloat16 numbers whose sum it is, `plane` apart (an infinite one is alone; what is left of numbers
+// below 2^-110 may be too small for the third).
 __device__ __forceinline__ void store_h(float* h, int64_t at, int64_t, float sum) { h[at] = sum; }
 __device__ __forceinline__ void store_h(bf16* h, int64_t at, int64_t plane, float sum) {
   const bf16 high = from_f32<bf16>(sum);
-  const float rest = sum - to_f32(high);
+  const float left = sum - to_f32(high), rest = __builtin_isfinite(left) ? left : 0.f;
+  const bf16 mid = from_f32<bf16>(rest);
   h[at] = high;
-  h[plane + at] = from_f32<bf16>(__builtin_isfinite(rest) ? rest : 0.f);
+  h[plane + at] = mid;
+  h[2 * plane + at] = from_f32<bf16>(rest - to_f32(mid));
 }
 
 // h of 16 RT rows and 16 CT columns.
@@ -376,7 +379,7 @@ constexpr int kRow = 68;   // floats of a row of 64 in a wave's memory: so padde
 template <typename T, int RT, bool VEC>
 __device__ __forceinline__ bool expand_tile(const AdapterArgs& a, const T* h, int hstride, int64_t plane, int t0, int set, int sets, int pass,
                                             bool copy, uint4* stage, bool vec_out) {
-  constexpr int kLane = Frag<T>::kLane, kStep = 4 * kLane;   // (a step: 64 bytes of each row, one product; two for h's two numbers)
+  constexpr int kLane = Frag<T>::kLane, kStep = 4 * kLane;   // (a step: 64 bytes of each row, one product; three for h's three numbers)
   const int lane = threadIdx.x & 63, quad = lane >> 4, m = lane & 15;
   if (set >= sets) return false;
   int s = 0;
@@ -547,7 +550,7 @@ constexpr int kFewRows = 16, kFewRank = 16;
 template <typename T, Rows ROWS, bool VEC>
 __global__ __launch_bounds__(kWaves * 64, 2) void adapter_few_kernel(const AdapterArgs a, int sets, bool vec_out) {
   __shared__ uint4 lds[std::max(std::max(kStageRows<1, 1>, kStageParts<1, 1>), kWaves * kStageExpand<T, 1>)];
-  __shared__ uint4 h_lds[kFewRows * kFewRank * 4 / 16];
+  __shared__ uint4 h_lds[kFewRows * kFewRank * kTerms<T> * (int)sizeof(T) / 16];
   int s = 0, first_set = 0, block = blockIdx.x, here = 0;
   for (;; ++s) {
     here = (a.first[s + 1] - a.first[s] + 63) / 64;
@@ -676,6 +679,8 @@ using namespace ninfer;
 extern "C" int ninfer_adapter_few_rows() { return kFewRows; }
 extern "C" int ninfer_adapter_few_rank() { return kFewRank; }
 extern "C" int ninfer_adapter_args_bytes() { return (int)sizeof(AdapterArgs); }
+// Bytes of scratch for each of a row's S R numbers of h.
+extern "C" int ninfer_adapter_h_bytes(int dtype) { return dtype == kBF16 ? kTerms<bf16> * (int)sizeof(bf16) : kTerms<float> * (int)sizeof(float); }
 
 extern "C" int ninfer_adapter_add(const AdapterArgs* args, hipStream_t stream) {
   NINFER_REQUIRE(args, "adapter_add: no arguments");

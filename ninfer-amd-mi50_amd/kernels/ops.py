@@ -384,6 +384,8 @@ class HipOps:
         if (self.lib.ninfer_adapter_few_rows(), self.lib.ninfer_adapter_few_rank(), self.lib.ninfer_logprob_most()) != (
                 self.ADAPTER_FEW_ROWS, self.ADAPTER_FEW_RANK, self.LISTED_TOKENS):
             raise KernelError(f"{self.lib_path} and these bindings differ on what few rows and the most listed tokens are")
+        if any(self.lib.ninfer_adapter_h_bytes(code) != self.ADAPTER_H_BYTES[dt] for dt, code in _DT.items()):
+            raise KernelError(f"{self.lib_path} and these bindings differ on the scratch of adapters")
         self.lib.ninfer_logprob_scratch_bytes.restype = ctypes.c_longlong
         self.lib.ninfer_attention_workspace_floats.restype = ctypes.c_longlong
         self.lib.ninfer_event_create.restype = ctypes.c_void_p
@@ -2256,6 +2258,7 @@ class HipOps:
         return torch.cuda.current_stream(device).cuda_stream if _raw_stream is None else _raw_stream(device)
 
     ADAPTER_FEW_ROWS, ADAPTER_FEW_RANK = 16, 16   # the library's own
+    ADAPTER_H_BYTES = {torch.float32: 4, torch.bfloat16: 6}   # ... scratch for a number between the two products
 
     def adapter_add(self, x, a, b, scale, ranks, widths, row_adapter, out, base=None, single_rows=0):
         """Low-rank adapters of many requests beside a projection whose output `base` [T, N] is (None: `out`, in place): for
@@ -2300,9 +2303,9 @@ class HipOps:
         if (pb != po or ldb != ldo) and pb < end_o and po < end_b:
             raise KernelError("adapter_add: base and out overlap")
         self._here(dev)
-        h = None   # (few rows need no scratch)
+        h, of_row = None, slices * r * self.ADAPTER_H_BYTES[dt]   # (few rows need no scratch)
         if t > self.ADAPTER_FEW_ROWS or r > self.ADAPTER_FEW_RANK:
-            h = torch.empty(t * slices * r, dtype=torch.float32, device=x.device)
+            h = torch.empty(t * of_row, dtype=torch.uint8, device=x.device)
         first = [0, n, n, n, n]
         for i in range(1, slices):
             first[i] = first[i - 1] + widths[i - 1]
@@ -2314,7 +2317,7 @@ class HipOps:
         apart = min(single_rows, count) >= 16 and t - single_rows >= 128
         for lo, hi in ((0, single_rows), (single_rows, t)) if apart else ((0, t),):
             args = _ADAPTER_ARGS.pack(px + lo * ldx * size, pa, p_b, p_scale, p_ranks, p_rows + 4 * lo, pb + lo * ldb * size,
-                                      po + lo * ldo * size, ph + lo * slices * r * 4, ldx, ldb, ldo, hi - lo, k, r, slices, count, n, *first, code, hi <= single_rows)
+                                      po + lo * ldo * size, ph + lo * of_row, ldx, ldb, ldo, hi - lo, k, r, slices, count, n, *first, code, hi <= single_rows)
             if lib.ninfer_adapter_add(args, stream):
                 self._ok(-1)
 
