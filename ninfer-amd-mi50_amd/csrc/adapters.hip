@@ -22,8 +22,12 @@
 //
 // A tile's sums run in the same order however many rows the step has: every form cuts k among
 // eight waves in the same way, and a request's numbers do not depend on its company.
+//
+// Where a kernel holds the projection's sums in 32 bits itself (qkv_rope.hip), it asks for what the adapters add alone, in
+// 32 bits (outputs of a type of their own, without a base; rows without an adapter are not written).
 #include "common.h"
 #include <algorithm>
+#include <type_traits>
 
 namespace ninfer {
 
@@ -34,7 +38,7 @@ struct AdapterArgs {
   const float* scale;    // [L]
   const int* ranks;      // [L]: rows of A (and columns of B) that count, clamped to [0, R]
   const int* row_adapter;   // [T]; outside [0, L): none
-  const void* base;      // [T, ldb]; may be out
+  const void* base;      // [T, ldb]; may be out; not read where the adapters' part is asked for alone
   void* out;             // [T, ldo]
   void* h;               // [T, S R] 32-bit numbers, or as many bfloat16 ones in each of three planes (kTerms)
   long long ldx, ldb, ldo;
@@ -375,10 +379,12 @@ __global__ __launch_bounds__(kWaves * 64, RT == 1 ? 4 : 2) void adapter_shrink_k
 constexpr int kRow = 68;   // floats of a row of 64 in a wave's memory: so padded that rows' columns lie in different banks
 
 // 16 RT rows from t0 on and the `set`th 64 columns, by one wave: what the tile's `pass`th adapter adds to its rows; with `copy` the
-// rows without an adapter too. h: all slices' numbers of row 0, rows `hstride` apart. False: the tile has no such adapter.
-template <typename T, int RT, bool VEC>
+// rows without an adapter too. h: all slices' numbers of row 0, rows `hstride` apart. False: the tile has no such adapter. With outputs
+// of another type than the rows' they are the adapter's part alone.
+template <typename T, int RT, bool VEC, typename O = T>
 __device__ __forceinline__ bool expand_tile(const AdapterArgs& a, const T* h, int hstride, int64_t plane, int t0, int set, int sets, int pass,
                                             bool copy, uint4* stage, bool vec_out) {
+  constexpr bool kAlone = !std::is_same<T, O>::value;
   constexpr int kLane = Frag<T>::kLane, kStep = 4 * kLane;   // (a step: 64 bytes of each row, one product; three for h's three numbers)
   const int lane = threadIdx.x & 63, quad = lane >> 4, m = lane & 15;
   if (set >= sets) return false;
@@ -389,16 +395,16 @@ __device__ __forceinline__ bool expand_tile(const AdapterArgs& a, const T* h, in
     set -= here;
   }
   const int c0 = a.first[s] + set * 64, end = a.first[s + 1], n = min(end - c0, 64);
-  const T* base = (const T*)a.base + c0;
-  T* out = (T*)a.out + c0;
+  const T* base = kAlone ? nullptr : (const T*)a.base + c0;
+  O* out = (O*)a.out + c0;
   h += s * a.R;
 
   // Rows as they lie in memory: 16 bytes a lane, kCols of them side by side.
-  constexpr int kEach = 16 / sizeof(T), kCols = 64 / kEach, kRows = 64 / kCols;
+  constexpr int kEach = 16 / sizeof(O), kCols = 64 / kEach, kRows = 64 / kCols;
   const bool whole = vec_out && n == 64;
   uint4 was[RT][16 / kRows];
   auto load_base = [&](unsigned long long rows) {
-    if (!whole) return;
+    if (kAlone || !whole) return;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -413,11 +419,16 @@ __device__ __forceinline__ bool expand_tile(const AdapterArgs& a, const T* h, in
       for (int i = 0; i < 16 / kRows; ++i) {
         const int in = i * kRows + lane / kCols, r = rt * 16 + in;
         if (!(rows >> r & 1)) continue;
-        T e[kEach];
-        __builtin_memcpy(e, &was[rt][i], 16);
-        if (tile_) {
+        O e[kEach];
+        if (kAlone) {
 #pragma unroll
-          for (int c = 0; c < kEach; ++c) e[c] = from_f32<T>(to_f32(e[c]) + scale * tile_[in * kRow + lane % kCols * kEach + c]);
+          for (int c = 0; c < kEach; ++c) e[c] = from_f32<O>(scale * tile_[in * kRow + lane % kCols * kEach + c]);
+        } else {
+          __builtin_memcpy(e, &was[rt][i], 16);
+          if (tile_) {
+#pragma unroll
+            for (int c = 0; c < kEach; ++c) e[c] = from_f32<O>(to_f32(e[c]) + scale * tile_[in * kRow + lane % kCols * kEach + c]);
+          }
         }
         uint4 v;
         __builtin_memcpy(&v, e, 16);
@@ -428,8 +439,12 @@ __device__ __forceinline__ bool expand_tile(const AdapterArgs& a, const T* h, in
       for (int in = 0; in < 16; ++in) {
         const int r = rt * 16 + in;
         if (!(rows >> r & 1) || lane >= n) continue;
-        const T v = base[(t0 + r) * a.ldb + lane];
-        out[(t0 + r) * a.ldo + lane] = tile_ ? from_f32<T>(to_f32(v) + scale * tile_[in * kRow + lane]) : v;
+        if constexpr (kAlone) {
+          out[(t0 + r) * a.ldo + lane] = from_f32<O>(scale * tile_[in * kRow + lane]);
+        } else {
+          const T v = base[(t0 + r) * a.ldb + lane];
+          out[(t0 + r) * a.ldo + lane] = tile_ ? from_f32<T>(to_f32(v) + scale * tile_[in * kRow + lane]) : v;
+        }
       }
     }
   };
@@ -519,7 +534,7 @@ __device__ __forceinline__ bool expand_tile(const AdapterArgs& a, const T* h, in
 template <typename T, int RT> constexpr int kStageExpand = std::max((4 + RT * kTerms<T>) * 64, 16 * kRow / 4);   // a wave's, in 16 bytes
 
 // Four waves take neighbouring columns. `more`: as in the other kernel.
-template <typename T, int RT, bool VEC>
+template <typename T, int RT, bool VEC, typename O = T>
 __global__ __launch_bounds__(kExpandWaves * 64, RT == 1 ? 4 : 3) void adapter_expand_kernel(const AdapterArgs a, int sets, int groups, int total, int more,
                                                                            bool vec_out) {
   __shared__ uint4 lds[kExpandWaves][kStageExpand<T, RT>];
@@ -534,8 +549,8 @@ __global__ __launch_bounds__(kExpandWaves * 64, RT == 1 ? 4 : 3) void adapter_ex
       group = further % groups;
       further += more;
     }
-    const bool had = expand_tile<T, RT, VEC>(a, (const T*)a.h, a.S * a.R, (int64_t)a.T * a.S * a.R, tile * (16 * RT), group * kExpandWaves + wave, sets, pass, pass == 0 && a.base != a.out,
-                                             lds[wave], vec_out);
+    const bool had = expand_tile<T, RT, VEC, O>(a, (const T*)a.h, a.S * a.R, (int64_t)a.T * a.S * a.R, tile * (16 * RT), group * kExpandWaves + wave, sets, pass,
+                                                std::is_same<T, O>::value && pass == 0 && a.base != a.out, lds[wave], vec_out);
     if (further < 0 && (more || !had)) return;
   }
 }
@@ -547,7 +562,7 @@ __global__ __launch_bounds__(kExpandWaves * 64, RT == 1 ? 4 : 3) void adapter_ex
 // 64, 3 x 2,048 columns, one row 10.4 and 9.1, 16 rows 14.1 and 11.5.
 constexpr int kFewRows = 16, kFewRank = 16;
 
-template <typename T, Rows ROWS, bool VEC>
+template <typename T, Rows ROWS, bool VEC, typename O = T>
 __global__ __launch_bounds__(kWaves * 64, 2) void adapter_few_kernel(const AdapterArgs a, int sets, bool vec_out) {
   __shared__ uint4 lds[std::max(std::max(kStageRows<1, 1>, kStageParts<1, 1>), kWaves * kStageExpand<T, 1>)];
   __shared__ uint4 h_lds[kFewRows * kFewRank * kTerms<T> * (int)sizeof(T) / 16];
@@ -578,8 +593,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void adapter_few_kernel(const Adapt
       });
       __syncthreads();
     }
-    expand_tile<T, 1, VEC>(a, h - s * a.R, stride, plane, 0, local < here ? first_set + local : sets, sets, pass,
-                           pass == 0 && a.base != a.out, lds + wave * kStageExpand<T, 1>, vec_out);
+    expand_tile<T, 1, VEC, O>(a, h - s * a.R, stride, plane, 0, local < here ? first_set + local : sets, sets, pass,
+                           std::is_same<T, O>::value && pass == 0 && a.base != a.out, lds + wave * kStageExpand<T, 1>, vec_out);
     if (g < 0) return;
     __syncthreads();   // (both memories are the next pass's)
   }
@@ -596,7 +611,7 @@ static dim3 grid_of(const AdapterArgs& a, int total, int* more) {
 }
 
 // How a call's rows can be read and written.
-template <typename T>
+template <typename T, typename O = T>
 struct Forms {
   bool x, b, out;   // 16 bytes at a time: x and A, B, base and out
   bool rest;        // x and A: with a rest behind the whole steps
@@ -606,17 +621,17 @@ struct Forms {
     x = four(a.x, a.ldx) && four(a.a, a.K);
     rest = a.K % (8 * Frag<T>::kLane) != 0;
     b = four(a.b, a.R);
-    out = four(a.base, a.ldb) && four(a.out, a.ldo);
+    out = std::is_same<T, O>::value ? four(a.base, a.ldb) && four(a.out, a.ldo) : (uintptr_t)a.out % 4 == 0;
     sets = 0;
     for (int s = 0; s < a.S; ++s) {
       sets += (a.first[s + 1] - a.first[s] + 63) / 64;
-      out &= a.first[s] * sizeof(T) % 4 == 0;
+      out &= a.first[s] * sizeof(O) % 4 == 0;
     }
   }
 };
 
-template <typename T, int RT, int CT>
-static void shrink(const AdapterArgs& a, const Forms<T>& f, hipStream_t stream) {
+template <typename T, int RT, int CT, typename O = T>
+static void shrink(const AdapterArgs& a, const Forms<T, O>& f, hipStream_t stream) {
   const int groups = (a.S * a.R + CT * 16 - 1) / (CT * 16), total = (a.T + 16 * RT - 1) / (16 * RT) * groups;
   int more = 0;
   const dim3 grid = grid_of<RT>(a, total, &more);
@@ -625,23 +640,23 @@ static void shrink(const AdapterArgs& a, const Forms<T>& f, hipStream_t stream) 
   else adapter_shrink_kernel<T, RT, CT, kWhole><<<grid, kWaves * 64, 0, stream>>>(a, groups, total, more);
 }
 
-template <typename T, int RT>
-static void expand(const AdapterArgs& a, const Forms<T>& f, hipStream_t stream) {
+template <typename T, int RT, typename O = T>
+static void expand(const AdapterArgs& a, const Forms<T, O>& f, hipStream_t stream) {
   const int groups = (f.sets + kExpandWaves - 1) / kExpandWaves, total = (a.T + 16 * RT - 1) / (16 * RT) * groups;
   int more = 0;
   const dim3 grid = grid_of<RT>(a, total, &more);
-  if (f.b) adapter_expand_kernel<T, RT, true><<<grid, kExpandWaves * 64, 0, stream>>>(a, f.sets, groups, total, more, f.out);
-  else adapter_expand_kernel<T, RT, false><<<grid, kExpandWaves * 64, 0, stream>>>(a, f.sets, groups, total, more, f.out);
+  if (f.b) adapter_expand_kernel<T, RT, true, O><<<grid, kExpandWaves * 64, 0, stream>>>(a, f.sets, groups, total, more, f.out);
+  else adapter_expand_kernel<T, RT, false, O><<<grid, kExpandWaves * 64, 0, stream>>>(a, f.sets, groups, total, more, f.out);
 }
 
-template <typename T>
-static void few(const AdapterArgs& a, const Forms<T>& f, hipStream_t stream) {
+template <typename T, typename O = T>
+static void few(const AdapterArgs& a, const Forms<T, O>& f, hipStream_t stream) {
   int blocks = 0;
   for (int s = 0; s < a.S; ++s) blocks += ((a.first[s + 1] - a.first[s] + 63) / 64 + kWaves - 1) / kWaves;
   const dim3 grid(blocks, std::min(a.T, a.L));
-  if (!f.x || !f.b) adapter_few_kernel<T, kSingle, false><<<grid, kWaves * 64, 0, stream>>>(a, f.sets, f.out);
-  else if (f.rest) adapter_few_kernel<T, kRest, true><<<grid, kWaves * 64, 0, stream>>>(a, f.sets, f.out);
-  else adapter_few_kernel<T, kWhole, true><<<grid, kWaves * 64, 0, stream>>>(a, f.sets, f.out);
+  if (!f.x || !f.b) adapter_few_kernel<T, kSingle, false, O><<<grid, kWaves * 64, 0, stream>>>(a, f.sets, f.out);
+  else if (f.rest) adapter_few_kernel<T, kRest, true, O><<<grid, kWaves * 64, 0, stream>>>(a, f.sets, f.out);
+  else adapter_few_kernel<T, kWhole, true, O><<<grid, kWaves * 64, 0, stream>>>(a, f.sets, f.out);
 }
 
 // Blocks of 32 rows and 64 columns of the first product from which these are the faster ones: blocks of 16 by 16 are many more. us of both
@@ -671,6 +686,15 @@ static void launch(const AdapterArgs& a, hipStream_t stream) {
   else expand<T, 1>(a, f, stream);
 }
 
+// The adapters' part alone: rows of few steps, in the tiles of 16 rows.
+template <typename T, typename O>
+static void launch_alone(const AdapterArgs& a, hipStream_t stream) {
+  const Forms<T, O> f(a);
+  if (a.T <= kFewRows && a.R <= kFewRank) return few<T, O>(a, f, stream);
+  shrink<T, 1, 1, O>(a, f, stream);
+  expand<T, 1, O>(a, f, stream);
+}
+
 }  // namespace ninfer
 
 using namespace ninfer;
@@ -682,24 +706,37 @@ extern "C" int ninfer_adapter_args_bytes() { return (int)sizeof(AdapterArgs); }
 // Bytes of scratch for each of a row's S R numbers of h.
 extern "C" int ninfer_adapter_h_bytes(int dtype) { return dtype == kBF16 ? kTerms<bf16> * (int)sizeof(bf16) : kTerms<float> * (int)sizeof(float); }
 
-extern "C" int ninfer_adapter_add(const AdapterArgs* args, hipStream_t stream) {
+static int check_adapters(const AdapterArgs* args, bool alone) {
   NINFER_REQUIRE(args, "adapter_add: no arguments");
   const AdapterArgs& a = *args;
   NINFER_REQUIRE(a.T > 0 && a.K > 0 && a.R > 0 && a.L > 0, "adapter_add: T=%d K=%d R=%d L=%d must be positive", a.T, a.K, a.R, a.L);
   NINFER_REQUIRE(a.S >= 1 && a.S <= 4 && a.first[0] == 0 && a.first[a.S] == a.N, "adapter_add: %d slices of %d columns", a.S, a.N);
   for (int s = 0; s < a.S; ++s)
     NINFER_REQUIRE(a.first[s] < a.first[s + 1], "adapter_add: slice %d has no columns", s);
-  NINFER_REQUIRE(a.x && a.a && a.b && a.scale && a.ranks && a.row_adapter && a.base && a.out && (a.h || (a.T <= kFewRows && a.R <= kFewRank)),
-                 "adapter_add: a required array is null");
-  NINFER_REQUIRE(a.ldx >= a.K && a.ldb >= a.N && a.ldo >= a.N, "adapter_add: a row stride is less than the row");
-  NINFER_REQUIRE(a.base != a.out || a.ldb == a.ldo, "adapter_add: in place with two row strides");
+  NINFER_REQUIRE(a.x && a.a && a.b && a.scale && a.ranks && a.row_adapter && (a.base || alone) && a.out &&
+                     (a.h || (a.T <= kFewRows && a.R <= kFewRank)), "adapter_add: a required array is null");
+  NINFER_REQUIRE(a.ldx >= a.K && (alone || a.ldb >= a.N) && a.ldo >= a.N, "adapter_add: a row stride is less than the row");
+  NINFER_REQUIRE(alone || a.base != a.out || a.ldb == a.ldo, "adapter_add: in place with two row strides");
   // (threads of a grid's x, in blocks of 16 rows: 512 for 16 columns of h, 64 for 64 of out)
   const long long tiles = (a.T + 15ll) / 16;
   NINFER_REQUIRE(a.S * (long long)a.R <= 0x7fffffff && tiles * ((a.S * a.R + 15ll) / 16) * 512 <= 0x7fffffffll &&
                      tiles * (a.N / 64 + 8ll) * 64 <= 0x7fffffffll, "adapter_add: %d rows are too many", a.T);
-  NINFER_REQUIRE(a.dtype == kF32 || a.dtype == kBF16, "adapter_add: dtype %d", a.dtype);
-  if (a.dtype == kBF16) launch<bf16>(a, stream);
-  else launch<float>(a, stream);
+  NINFER_REQUIRE(a.dtype == kBF16 || (a.dtype == kF32 && !alone), "adapter_add: dtype %d", a.dtype);
+  return 0;
+}
+
+extern "C" int ninfer_adapter_add(const AdapterArgs* args, hipStream_t stream) {
+  if (const int rc = check_adapters(args, false)) return rc;
+  if (args->dtype == kBF16) launch<bf16>(*args, stream);
+  else launch<float>(*args, stream);
+  NINFER_LAUNCH_CHECK();
+  return 0;
+}
+
+// What the adapters add to bfloat16 rows alone, in 32 bits: out [T, ldo] of 32-bit numbers, of rows that have an adapter.
+extern "C" int ninfer_adapter_rows(const AdapterArgs* args, hipStream_t stream) {
+  if (const int rc = check_adapters(args, true)) return rc;
+  launch_alone<bf16, float>(*args, stream);
   NINFER_LAUNCH_CHECK();
   return 0;
 }

@@ -11,6 +11,8 @@
 // src/ops/kernels.hip:86-91), so that the block's epilogue holds both elements
 // of every pair it rotates. Angles, cosines and sines are 32-bit
 // (pos * inv_freq[i], sincosf), as in the rotation kernel of elementwise.hip.
+// What requests' low-rank adapters add to their rows (adapters.hip makes it, in 32 bits) joins the 32-bit
+// sums there too, so that rows without an adapter keep their bits beside rows that have one.
 // The reference fuses rotation and cache write into its one-row GEMV the same
 // way (src/ops/gemv.hip:271-324).
 #include "gemm.h"
@@ -40,6 +42,9 @@ struct QkvRopeArgs {
   int bt_stride;
   int page_size;
   int write_kv;           // 0: a layer that reads another layer's cache writes q only
+  const float* add;       // [T, (Hq + 2 Hkv) D]: to the products of rows that have an adapter; or null
+  const int* row_adapter; // [T]: a row's adapter; outside [0, adapters): it has none, and its row of `add` is not used
+  int adapters;
 };
 
 template <int WAVES>
@@ -116,18 +121,28 @@ __global__ __launch_bounds__(WAVES * 64) void qkv_rope_kernel(QkvRopeArgs a, int
   // partial tiles -> LDS, element (weight row f, token m) at [m * 16 + f]
 #pragma unroll
   for (int v = 0; v < 4; ++v) red[wave][r * 16 + 4 * j + v] = acc[v];
+  // thread (m, p): pair p of row m
+  const int m = threadIdx.x >> 3, p = threadIdx.x & 7, row = row0 + m;
+  float add_lo = 0.f, add_hi = 0.f;
+  bool adds = false;
+  if (a.add && threadIdx.x < 128 && row < a.T && p < pairs) {
+    const float* add = a.add + (int64_t)row * (a.Hq + 2 * a.Hkv) * D + head * D + d0 + p;
+    add_lo = add[0], add_hi = add[half];   // (on their way while the waves wait for each other)
+    adds = (unsigned)a.row_adapter[row] < (unsigned)a.adapters;
+  }
   __syncthreads();
 
-  // thread (m, p): pair p of row m
   if (threadIdx.x < 128) {
-    const int m = threadIdx.x >> 3, p = threadIdx.x & 7;
-    const int row = row0 + m;
     if (row < a.T && p < pairs) {
       float lo = 0.f, hi = 0.f;
 #pragma unroll
       for (int w = 0; w < WAVES; ++w) {
         lo += red[w][m * 16 + p];
         hi += red[w][m * 16 + 8 + p];
+      }
+      if (adds) {
+        lo += add_lo;
+        hi += add_hi;
       }
       const int d = d0 + p;
       if (a.bias) {
@@ -177,6 +192,7 @@ extern "C" int ninfer_qkv_rope(const QkvRopeArgs* args, hipStream_t stream) {
                  a.K, a.lda, a.D);
   NINFER_REQUIRE(a.Hq > 0 && a.Hkv > 0 && a.page_size > 0 && a.bt_stride > 0,
                  "qkv_rope: bad head counts, page size or table width");
+  NINFER_REQUIRE(!a.add || (a.row_adapter && a.adapters > 0), "qkv_rope: rows to add without the rows' adapters");
   NINFER_REQUIRE(((uintptr_t)a.x % 16 == 0) && ((uintptr_t)a.w % 16 == 0),
                  "qkv_rope: operands must be 16-byte aligned");
   const int heads = a.write_kv ? a.Hq + 2 * a.Hkv : a.Hq;

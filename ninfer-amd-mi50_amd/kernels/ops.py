@@ -198,7 +198,7 @@ class _QkvRopeArgs(ctypes.Structure):
                 ("block_table", ctypes.c_void_p), ("T", ctypes.c_int), ("K", ctypes.c_int),
                 ("lda", ctypes.c_int), ("Hq", ctypes.c_int), ("Hkv", ctypes.c_int),
                 ("D", ctypes.c_int), ("bt_stride", ctypes.c_int), ("page_size", ctypes.c_int),
-                ("write_kv", ctypes.c_int)]
+                ("write_kv", ctypes.c_int), ("add", ctypes.c_void_p), ("row_adapter", ctypes.c_void_p), ("adapters", ctypes.c_int)]
 
 
 class _LatentArgs(ctypes.Structure):
@@ -393,7 +393,7 @@ class HipOps:
         self.lib.ninfer_sample_spread_bytes.restype = ctypes.c_longlong
         p, i = ctypes.c_void_p, ctypes.c_int
         self.lib.ninfer_gemm.argtypes = [p, i, p]
-        self.lib.ninfer_adapter_add.argtypes = self.lib.ninfer_adjust_logits.argtypes = [ctypes.c_char_p, p]
+        self.lib.ninfer_adapter_add.argtypes = self.lib.ninfer_adapter_rows.argtypes = self.lib.ninfer_adjust_logits.argtypes = [ctypes.c_char_p, p]
         self.lib.ninfer_token_logprobs.argtypes = [ctypes.c_char_p, p, p]
         self.lib.ninfer_sample_rows.argtypes = [p, i, i, i, i, p, p, ctypes.c_longlong, i, p, p, p]
         self.lib.ninfer_latent_attention_workspace_floats.restype = ctypes.c_longlong
@@ -666,17 +666,17 @@ class HipOps:
 
     def qkv_rope(self, x, w_qkv, bias, qkv, positions, row_seq, inv_freq, rot_dim, n_q, n_kv,
                  head_dim, k_pool, v_pool, block_table, page_size, write_kv=True,
-                 interleaved=False, q_norm=None, k_norm=None, norm_eps=0.0):
+                 interleaved=False, q_norm=None, k_norm=None, norm_eps=0.0, adapters=None):
         """qkv = x w_qkv^T, then what `rope_kv_write` does. Few bf16 rows with a full
         rotation in half-split pairs and no norm of the heads run as one kernel (its blocks
-        hold parts of heads); everything else as the product and the rotation kernel one after
-        the other."""
+        hold parts of heads; see `qkv_rope_takes`); everything else as the product and the rotation kernel one after
+        the other. `adapters`: (a, b, scale, ranks, widths, row_adapter, single_rows) as `adapter_add` takes them: what the
+        rows' adapters add to the product before its bias. Rows without an adapter keep the bits that they have without `adapters`."""
         t = x.shape[0]
-        fused = (not self.force_generic and not interleaved and x.dtype == torch.bfloat16
-                 and x.dim() == 2 and q_norm is None
-                 and self.lib.ninfer_qkv_rope_takes(t, x.shape[1], x.shape[1], head_dim, rot_dim))
-        if not fused:
+        if not self.qkv_rope_takes(x, head_dim, rot_dim, interleaved, q_norm):
             self.linear(x, w_qkv, qkv)
+            if adapters is not None:
+                self.adapter_add(x, *adapters[:6], qkv, single_rows=adapters[6])
             self.rope_kv_write(qkv, bias, positions, row_seq, inv_freq, rot_dim, n_q, n_kv,
                                head_dim, k_pool, v_pool, block_table, page_size, write_kv,
                                interleaved, q_norm, k_norm, norm_eps)
@@ -699,12 +699,24 @@ class HipOps:
         _need(k_pool.shape == v_pool.shape and k_pool.shape[1:] == (n_kv, page_size, head_dim),
               "qkv_rope: pools do not fit the head layout")
         _dev(block_table, "block_table", torch.int32, 2)
+        add = None
+        if adapters is not None:
+            _need(adapters[1].dim() == 3 and adapters[1].shape[1] == width, "qkv_rope: the adapters' columns are not the product's")
+            add = self._adapter_rows(x, *adapters[:6])
         args = _QkvRopeArgs(x.data_ptr(), w_qkv.data_ptr(), _ptr(bias), qkv.data_ptr(),
                             positions.data_ptr(), row_seq.data_ptr(), inv_freq.data_ptr(),
                             k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(), t,
                             x.shape[1], x.shape[1], n_q, n_kv, head_dim, block_table.shape[1],
                             page_size, 1 if write_kv else 0)
+        if add is not None:
+            args.add, args.row_adapter, args.adapters = add.data_ptr(), adapters[5].data_ptr(), adapters[1].shape[0]
         self._ok(self.lib.ninfer_qkv_rope(ctypes.byref(args), self._stream()))
+
+    def qkv_rope_takes(self, x, head_dim, rot_dim, interleaved=False, q_norm=None) -> bool:
+        """Does `qkv_rope` run these rows as one kernel, which holds the products in 32 bits until they have turned?"""
+        return bool(not self.force_generic and not interleaved and x.dtype == torch.bfloat16
+                    and x.dim() == 2 and q_norm is None
+                    and self.lib.ninfer_qkv_rope_takes(x.shape[0], x.shape[1], x.shape[1], head_dim, rot_dim))
 
     def moe_combine(self, residual, y, wts, shared=None, gate=None):
         _dev(residual, "residual", torch.float32, 2)
@@ -2269,57 +2281,80 @@ class HipOps:
         count, whatever it holds. Rows whose number is outside [0, L) have no adapter: out = base. `single_rows`: the first
         so many rows are of different requests each, as a step has them; many other rows should be
         neighbours where they share an adapter. It changes the time alone: a row's numbers are the same in any company."""
-        dt = x.dtype
-        if dt not in _DT:
-            raise KernelError(f"adapter_add: rows of {dt}")
         in_place = base is None or base is out
-        ldx, ldo = self._rows_of(x, dt, "adapter_add: x"), self._rows_of(out, dt, "adapter_add: out")
+        dt, t, n, dev, size, tables, p_rows, shape = self._adapter_tables(x, a, b, scale, ranks, widths, row_adapter)
+        ldo = self._rows_of(out, dt, "adapter_add: out")
         ldb = ldo if in_place else self._rows_of(base, dt, "adapter_add: base")
-        dev = x.get_device()
-        (t, k), slices = x.shape, len(widths)
-        if not (a.dtype is dt and b.dtype is dt and a.dim() == 3 and b.dim() == 3 and a.is_contiguous() and b.is_contiguous()
-                and a.get_device() == dev and b.get_device() == dev and out.get_device() == dev):
-            raise KernelError(f"adapter_add: factors must be three-dimensional, contiguous and of {dt}, on the rows' GPU")
-        count, n, r = b.shape
-        if not (1 <= slices <= 4 and min(widths) >= 1 and sum(widths) == n and a.shape == (count, slices * r, k) and count and r and k):
-            raise KernelError(f"adapter_add: factors {tuple(a.shape)} and {tuple(b.shape)} do not fit {k} columns and slices {tuple(widths)}")
-        if out.shape != (t, n) or not (in_place or (base.shape == (t, n) and base.get_device() == dev)):
+        if out.shape != (t, n) or out.get_device() != dev or not (in_place or (base.shape == (t, n) and base.get_device() == dev)):
             raise KernelError(f"adapter_add: out and base must be [{t}, {n}], on the rows' GPU")
-        p_scale = self._flat(scale, torch.float32, count, dev, "adapter_add: scale")
-        p_ranks = self._flat(ranks, torch.int32, count, dev, "adapter_add: ranks")
-        p_rows = self._flat(row_adapter, torch.int32, t, dev, "adapter_add: row_adapter")
         if not 0 <= single_rows <= t:
             raise KernelError(f"adapter_add: {single_rows} single rows of {t}")
-        if self._held is not None:
-            raise KernelError("adapter_add: inside together(), where products have not been launched")
         if t == 0:
             return
+        (ldx, k, r, slices, count), first = shape
         px, po = x.data_ptr(), out.data_ptr()
         pb = po if in_place else base.data_ptr()
-        size = 4 if dt is torch.float32 else 2
         end_x, end_o, end_b = (p + ((t - 1) * ld + w) * size for p, ld, w in ((px, ldx, k), (po, ldo, n), (pb, ldb, n)))
         if px < end_o and po < end_x:
             raise KernelError("adapter_add: x and out overlap")
         if (pb != po or ldb != ldo) and pb < end_o and po < end_b:
             raise KernelError("adapter_add: base and out overlap")
         self._here(dev)
-        h, of_row = None, slices * r * self.ADAPTER_H_BYTES[dt]   # (few rows need no scratch)
-        if t > self.ADAPTER_FEW_ROWS or r > self.ADAPTER_FEW_RANK:
-            h = torch.empty(t * of_row, dtype=torch.uint8, device=x.device)
-        first = [0, n, n, n, n]
-        for i in range(1, slices):
-            first[i] = first[i - 1] + widths[i - 1]
-        lib, stream, code = self.lib, self._stream_of(dev), _DT[dt]
-        pa, p_b, ph = a.data_ptr(), b.data_ptr(), 0 if h is None else h.data_ptr()
+        h, of_row = self._adapter_scratch(x, slices, r)
+        lib, stream, code, ph = self.lib, self._stream_of(dev), _DT[dt], 0 if h is None else h.data_ptr()
         # (Single rows of many adapters beside other rows: two calls, since a tile of theirs has an adapter a row. us so and in one call, 64
         # adapters of rank 16 beside q, k and v of 2,048 columns: 32 of them and 512 rows 27 and 39, 2,048 rows 39 and 49; 8 of them 21 and
         # 16, 34 and 30.)
         apart = min(single_rows, count) >= 16 and t - single_rows >= 128
         for lo, hi in ((0, single_rows), (single_rows, t)) if apart else ((0, t),):
-            args = _ADAPTER_ARGS.pack(px + lo * ldx * size, pa, p_b, p_scale, p_ranks, p_rows + 4 * lo, pb + lo * ldb * size,
-                                      po + lo * ldo * size, ph + lo * of_row, ldx, ldb, ldo, hi - lo, k, r, slices, count, n, *first, code, hi <= single_rows)
+            args = _ADAPTER_ARGS.pack(px + lo * ldx * size, *tables, p_rows + 4 * lo, pb + lo * ldb * size, po + lo * ldo * size,
+                                      ph + lo * of_row, ldx, ldb, ldo, hi - lo, k, r, slices, count, n, *first, code, hi <= single_rows)
             if lib.ninfer_adapter_add(args, stream):
                 self._ok(-1)
+
+    def _adapter_tables(self, x, a, b, scale, ranks, widths, row_adapter):
+        """What every call with adapters checks of its rows and tables: (type, rows, columns, device, bytes of a number, addresses of a,
+        b, scale and ranks, that of row_adapter, ((row stride, K, R, slices, L), the slices' first columns))."""
+        dt = x.dtype
+        if dt not in _DT:
+            raise KernelError(f"adapter_add: rows of {dt}")
+        ldx, dev = self._rows_of(x, dt, "adapter_add: x"), x.get_device()
+        (t, k), slices = x.shape, len(widths)
+        if not (a.dtype is dt and b.dtype is dt and a.dim() == 3 and b.dim() == 3 and a.is_contiguous() and b.is_contiguous()
+                and a.get_device() == dev and b.get_device() == dev):
+            raise KernelError(f"adapter_add: factors must be three-dimensional, contiguous and of {dt}, on the rows' GPU")
+        count, n, r = b.shape
+        if not (1 <= slices <= 4 and min(widths) >= 1 and sum(widths) == n and a.shape == (count, slices * r, k) and count and r and k):
+            raise KernelError(f"adapter_add: factors {tuple(a.shape)} and {tuple(b.shape)} do not fit {k} columns and slices {tuple(widths)}")
+        tables = (a.data_ptr(), b.data_ptr(), self._flat(scale, torch.float32, count, dev, "adapter_add: scale"),
+                  self._flat(ranks, torch.int32, count, dev, "adapter_add: ranks"))
+        p_rows = self._flat(row_adapter, torch.int32, t, dev, "adapter_add: row_adapter")
+        if self._held is not None:
+            raise KernelError("adapter_add: inside together(), where products have not been launched")
+        first = [0, n, n, n, n]
+        for i in range(1, slices):
+            first[i] = first[i - 1] + widths[i - 1]
+        return dt, t, n, dev, 4 if dt is torch.float32 else 2, tables, p_rows, ((ldx, k, r, slices, count), first)
+
+    def _adapter_scratch(self, x, slices, r):
+        """(scratch for the first product of x's rows, or None: few rows need none; its bytes a row)"""
+        of_row = slices * r * self.ADAPTER_H_BYTES[x.dtype]
+        if x.shape[0] <= self.ADAPTER_FEW_ROWS and r <= self.ADAPTER_FEW_RANK:
+            return None, of_row
+        return torch.empty(x.shape[0] * of_row, dtype=torch.uint8, device=x.device), of_row
+
+    def _adapter_rows(self, x, a, b, scale, ranks, widths, row_adapter):
+        """What the adapters of bfloat16 rows add, alone, in 32 bits [T, N]; rows without an adapter hold anything."""
+        dt, t, n, dev, _, tables, p_rows, (shape, first) = self._adapter_tables(x, a, b, scale, ranks, widths, row_adapter)
+        self._here(dev)
+        out = torch.empty_strided((t, n), (n, 1), dtype=torch.float32, device=x.device)
+        ldx, k, r, slices, count = shape
+        h, _ = self._adapter_scratch(x, slices, r)
+        args = _ADAPTER_ARGS.pack(x.data_ptr(), *tables, p_rows, 0, out.data_ptr(), 0 if h is None else h.data_ptr(), ldx, 0, n,
+                                  t, k, r, slices, count, n, *first, _DT[dt], 0)
+        if self.lib.ninfer_adapter_rows(args, self._stream_of(dev)):
+            self._ok(-1)
+        return out
 
     def adjust_logits(self, logits, out=None, *, repetition=None, presence=None, frequency=None, hist_offsets=None,
                       hist_tokens=None, hist_counts=None, hist_generated=None, bias_offsets=None, bias_tokens=None,

@@ -27,8 +27,8 @@ learned number per head (`sink="learned"`). Such a layer reads its input through
 product (`input_width`), which layers side by side may share.
 
 Requests may have low-rank adapters beside the projections (`adapter_spots`): beside q, k, v (and
-the output gate), which are one product, and beside the output projection. A step in which a request has
-one runs the product, the adapters and the rotation one after the other.
+the output gate), which are one product, and beside the output projection. Where product, rotation and cache write are one
+kernel, it takes what the adapters add in 32 bits; elsewhere the product, the adapters and the rotation run one after the other.
 """
 from __future__ import annotations
 
@@ -346,8 +346,11 @@ class Attention(Mixer):
                  self.head_dim, cache["k"], cache["v"], cache.block_table, cache.page_size)
         how = dict(write_kv=call.writes_cache, interleaved=self.position.pairing == "interleaved",
                    q_norm=self.q_norm, k_norm=self.k_norm, norm_eps=self.qk_norm_eps or 0.0)
-        if ctx.row_adapter is None:
+        given = self.spot_in.given(ctx)
+        if given is None:
             ops.qkv_rope(x, self.w_qkv, self.b_qkv, qkv, *where, **how)
+        elif hasattr(ops, "qkv_rope_takes"):   # (rows without an adapter keep the bits that they have without the others')
+            ops.qkv_rope(x, self.w_qkv, self.b_qkv, qkv, *where, **how, adapters=given)
         else:
             ops.linear(x, self.w_qkv, qkv)
             self.spot_in.add(ctx, x, qkv)

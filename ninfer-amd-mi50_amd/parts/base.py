@@ -249,9 +249,17 @@ class AdapterSpot:
 
     def add(self, ctx: "StepContext", x: torch.Tensor, out: torch.Tensor) -> None:
         """What the adapters of the step's rows add to the product's rows `out` of x, in place."""
-        if ctx.row_adapter is not None and self.tables is not None:
-            t = self.tables
-            ctx.ops.adapter_add(x, t.a, t.b, t.scale, t.ranks, t.widths, ctx.row_adapter, out, single_rows=ctx.single_rows)
+        given = self.given(ctx)
+        if given is not None:
+            ctx.ops.adapter_add(x, *given[:6], out, single_rows=given[6])
+
+    def given(self, ctx: "StepContext") -> Optional[tuple]:
+        """The step's adapters at this spot as calls take them (factors, scales, ranks, widths, the rows' numbers, single rows), or
+        None: no row of the step has one."""
+        if ctx.row_adapter is None or self.tables is None:
+            return None
+        t = self.tables
+        return t.a, t.b, t.scale, t.ranks, t.widths, ctx.row_adapter, ctx.single_rows
 
 
 @dataclass
