@@ -9,10 +9,28 @@ generated, by the second if it was at all), `logit_bias` (token id -> what is ad
 from __future__ import annotations
 
 import math
+import operator
+from collections.abc import Mapping
 from dataclasses import dataclass
 from typing import Dict, Optional
 
 _MOST = 3.4028234663852886e38   # the largest 32-bit float
+
+
+def _number(value) -> float:
+    """`value`, NaN for what is no number."""
+    try:
+        return math.nan if isinstance(value, (str, bytes)) else float(value)
+    except (TypeError, ValueError, OverflowError):
+        return math.nan
+
+
+def _count(value) -> int:
+    """`value`, -1 for what is no whole number."""
+    try:
+        return operator.index(value)
+    except TypeError:
+        return -1
 
 
 @dataclass
@@ -29,17 +47,23 @@ class SamplingParams:
     logprobs: Optional[int] = None
 
     def check(self, vocab: int, most_listed: int) -> None:
-        """ValueError for what no row of `vocab` logits can be asked for."""
+        """ValueError for what no row of `vocab` logits can be asked for, and for options that are no numbers."""
         for name in ("presence_penalty", "frequency_penalty"):
-            if not abs(getattr(self, name)) <= _MOST:
-                raise ValueError(f"{name} must be finite, is {getattr(self, name)}")
+            if not abs(_number(getattr(self, name))) <= _MOST:
+                raise ValueError(f"{name} must be finite, is {getattr(self, name)!r}")
+        if self.logit_bias and not isinstance(self.logit_bias, Mapping):
+            raise ValueError(f"logit_bias must be a dict of token ids and biases, is {self.logit_bias!r}")
         for token, bias in (self.logit_bias or {}).items():
-            if not 0 <= int(token) < vocab:
-                raise ValueError(f"logit_bias names token {token}, the vocabulary is [0, {vocab})")
-            if not (abs(bias) <= _MOST or bias == -math.inf):
-                raise ValueError(f"logit_bias of token {token} is {bias}")
-        if self.logprobs is not None and not 0 <= self.logprobs <= min(most_listed, vocab):
-            raise ValueError(f"logprobs must be in [0, {min(most_listed, vocab)}], is {self.logprobs}")
+            try:
+                fine = 0 <= int(token) < vocab
+            except (TypeError, ValueError, OverflowError):
+                fine = False
+            if not fine:
+                raise ValueError(f"logit_bias names token {token!r}, the vocabulary is [0, {vocab})")
+            if not (abs(_number(bias)) <= _MOST or _number(bias) == -math.inf):
+                raise ValueError(f"logit_bias of token {token} is {bias!r}")
+        if self.logprobs is not None and not 0 <= _count(self.logprobs) <= min(most_listed, vocab):
+            raise ValueError(f"logprobs must be in [0, {min(most_listed, vocab)}], is {self.logprobs!r}")
 
     @staticmethod
     def greedy(max_new_tokens: int = 512) -> "SamplingParams":
