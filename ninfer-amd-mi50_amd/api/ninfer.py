@@ -257,9 +257,13 @@ class Ninfer:
             stop_ids = list(self.runner.spec.eos_token_ids)
         sched = Scheduler(self.runner, self.sampler)
         reqs = [Request(str(i), list(p), q, stop_ids, a, f) for i, (p, q, a, f) in enumerate(zip(prompts, params, adapters, allow))]
-        for r in reqs:
-            sched.add(r)
-        sched.run()
+        try:
+            for r in reqs:
+                sched.add(r)
+            sched.run()
+        except BaseException as e:   # (the scheduler ends with this call: nothing may stay held by its requests)
+            sched.abort(str(e))
+            raise
         for r in reqs:
             if r.status == "failed":
                 raise RuntimeError(f"request {r.id}: {r.error}")

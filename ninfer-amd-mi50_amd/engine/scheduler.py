@@ -115,7 +115,7 @@ class Scheduler:
             return
         try:
             request.params.check(self.runner.vocab_size, getattr(self.runner.ops, "LISTED_TOKENS", 0))
-            self.runner.hold_adapter(request.adapter)
+            self.runner.adapter_number(request.adapter)
         except ValueError as e:
             request.status, request.error = "failed", str(e)
             self.finished.append(request)
@@ -129,6 +129,7 @@ class Scheduler:
         request.order = self._next_key
         self._next_key += 1
         request.history = History(request.prompt)
+        self.runner.hold_adapter(request.adapter)   # (last: whatever raises before it leaves nothing held)
         request.status = "waiting"
         self.waiting.append(request)
 
@@ -305,3 +306,18 @@ class Scheduler:
         while self.has_work():
             self.step()
         return self.finished
+
+    def abort(self, error: str = "aborted") -> List[Request]:
+        """Ends every request that is waiting or running as failed, and gives back its slot, pages and adapter: after a step that
+        raised, for whoever does not go on with it. Returns them."""
+        ended = self.running + list(self.waiting)
+        self.running, self.waiting = [], deque()
+        for req in ended:
+            self.runner.let_go_adapter(req.adapter)
+            req.status, req.error = "failed", req.error or error
+            self.finished.append(req)
+        for req in ended:
+            slot, req.slot = req.slot, None
+            if slot is not None:
+                self.cache.release(slot)
+        return ended

@@ -25,3 +25,54 @@ def test_options_that_are_no_numbers_fail_their_own_request(tiny, options, what)
     assert (bad.status, fine.status) == ("failed", "finished") and what in bad.error
     with pytest.raises(RuntimeError, match="request 0"):
         eng.generate([[1]], greedy(2, **options), [])
+
+
+def test_a_call_that_raises_leaves_nothing_held(tiny, tmp_path, monkeypatch):  # noqa: F811
+    """Slots, pages and adapters of requests that wait or run come back, whatever ends the call that made them."""
+    folder, cfg, _ = tiny
+    eng = engine(folder, max_adapters=1, num_sequences=2, num_pages=14)
+    path = adapters_of(tmp_path, cfg)["all"][0]
+    free = [g.allocator.free_pages for g in eng.runner.cache.groups]
+
+    def stops(out):
+        if len(out) == 2:
+            raise KeyboardInterrupt
+        return None
+
+    def no_rows(logits, rows):
+        raise ArithmeticError("rows")
+
+    for prompts, error, allow, sample in (
+            ([[1, 2], [9999], [3], [4]], ValueError, None, None),          # a step that refuses its tokens
+            ([[1, 2], [None, 3]], TypeError, None, None),                  # a prompt that is none
+            ([[1, 2], [5] * 30, [3], [4]], KeyboardInterrupt, [stops] * 4, None),
+            ([[1, 2], [5], [3]], ArithmeticError, None, no_rows)):
+        eng.load_adapter("all", path)
+        with monkeypatch.context() as m:
+            if sample is not None:
+                m.setattr(eng.sampler, "sample", sample)
+            with pytest.raises(error):
+                eng.generate(prompts, greedy(6), [], ["all"] * len(prompts), allow)
+        assert eng.runner.cache.free_slots == 2
+        assert [g.allocator.free_pages for g in eng.runner.cache.groups] == free
+        eng.remove_adapter("all")     # (refused while a request has it)
+    eng.runner.cache.check()
+    assert len(eng.generate([[1, 2], [3]], greedy(3), [])) == 2
+
+
+def test_a_scheduler_that_is_given_up(tiny, tmp_path):  # noqa: F811
+    from ninfer_amd import Request, Scheduler
+    folder, cfg, _ = tiny
+    eng = engine(folder, num_sequences=2)
+    eng.load_adapter("all", adapters_of(tmp_path, cfg)["all"][0])
+    sched = Scheduler(eng.runner, eng.sampler)
+    reqs = [Request(str(i), [1 + i, 2, 3], greedy(5), [], "all") for i in range(4)]
+    for r in reqs:
+        sched.add(r)
+    sched.step()
+    with pytest.raises(TypeError):
+        sched.add(Request("none", [None], greedy(5), [], "all"))
+    assert sched.abort("enough") == reqs and not sched.has_work()
+    assert [(r.status, r.error, r.slot) for r in reqs] == [("failed", "enough", None)] * 4 and sched.finished == reqs
+    assert eng.runner.cache.free_slots == 2 and sched.abort() == []
+    eng.remove_adapter("all")
