@@ -202,7 +202,7 @@ class Ninfer:
         """Stateless sampling of one row (reference src/api/ninfer_c_api.cpp:248-260;
         there the history is empty, here `recent` may carry it, and `generated` the tokens behind it that were
         generated, to which alone the presence and frequency penalties apply). `allowed`: what may come, token ids or
-        the words of a mask (None: every token)."""
+        the words of a mask (None: every token). ValueError where biases leave none of it."""
         import torch
         row = torch.as_tensor(np.asarray(logits, dtype=np.float32)).reshape(1, -1).to(
             self.runner.device)
@@ -215,7 +215,10 @@ class Ninfer:
         self._sample_calls += 1
         r = SampleRow(params, history, 0, 0 if seed else self._sample_calls,
                       seed or fresh_seed(), allowed_words(allowed, row.shape[1]))
-        return self.sampler.sample(row, [r])[0]
+        token = self.sampler.sample(row, [r])[0]
+        if r.changes and r.bars(token):
+            raise ValueError("no token is left that may come")
+        return token
 
     def close(self) -> None:
         """Give the model, its cache, its captured graphs and the kernels' workspaces back to

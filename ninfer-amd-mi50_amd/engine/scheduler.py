@@ -275,6 +275,8 @@ class Scheduler:
             asked = [req.params.logprobs for req in wanting if req.params.logprobs is not None]
             told = self.sampler.logprobs(logits, tokens, max(asked)) if asked else None
             for i, (req, tok) in enumerate(zip(wanting, tokens)):
+                if req.error is None and rows[i].changes and rows[i].bars(tok):
+                    req.error = "no token is left that may come"
                 if req.error is not None:
                     self._finish(req)
                     req.status = "failed"

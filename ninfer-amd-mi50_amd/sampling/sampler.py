@@ -14,6 +14,7 @@ their repetition penalty is then part of that pass.
 """
 from __future__ import annotations
 
+import math
 import os
 from array import array
 from dataclasses import dataclass
@@ -143,6 +144,14 @@ class SampleRow:
         self.key = key
         self.draw = draw
         self.seed = seed
+
+    def bars(self, token: int) -> bool:
+        """May this token not come? Of a row whose logits are all -inf once its request has changed them the sampling kernels
+        draw one all the same."""
+        if self.allowed is not None and not int(self.allowed[token // 32]) >> token % 32 & 1:
+            return True
+        bias = self.params.logit_bias
+        return bool(bias) and bias.get(token, bias.get(str(token))) == -math.inf   # (ids may be text, as JSON has them)
 
 
 def allowed_words(allowed, vocab: int) -> Optional[np.ndarray]:

@@ -76,3 +76,35 @@ def test_a_scheduler_that_is_given_up(tiny, tmp_path):  # noqa: F811
     assert [(r.status, r.error, r.slot) for r in reqs] == [("failed", "enough", None)] * 4 and sched.finished == reqs
     assert eng.runner.cache.free_slots == 2 and sched.abort() == []
     eng.remove_adapter("all")
+
+
+@pytest.mark.parametrize("temperature", [0.0, 1.0])
+def test_a_request_that_no_token_is_left_to_ends_itself(tiny, temperature):  # noqa: F811
+    """Masks and biases that together (or biases that alone) bar every token: no barred token comes."""
+    from ninfer_amd import Request, Scheduler
+    eng = engine(tiny[0])
+    every = {t: -INF for t in range(256)}
+    sched = Scheduler(eng.runner, eng.sampler)
+    draw = lambda **kw: greedy(4, temperature=temperature, seed=3, **kw)
+    reqs = [Request("a", [1, 2], draw(logit_bias={9: -INF}), allow=lambda out: [9]),
+            Request("b", [1, 2], draw(logit_bias={9: -INF, 8: 1.0}), allow=lambda out: [9, 8] if len(out) < 2 else [9]),
+            Request("c", [1, 2], draw(logit_bias=every)), Request("d", [1, 2], draw()),
+            Request("e", [1, 2], draw(logit_bias={str(t): -INF for t in range(256)})),
+            Request("f", [1, 2], draw(logit_bias={t: v for t, v in every.items() if t != 77}))]
+    for r in reqs:
+        sched.add(r)
+    sched.run()
+    assert [r.status for r in reqs] == ["failed", "failed", "failed", "finished", "failed", "finished"]
+    assert all("no token is left" in r.error for r in reqs if r.status == "failed")
+    assert [r.output for r in reqs[:3]] == [[], [8, 8], []] and reqs[4].output == [] and reqs[5].output == [77] * 4
+    assert eng.runner.cache.free_slots == 4
+    import numpy as np
+    row = np.zeros(256, np.float32)
+    for kw in (dict(allowed=[9, 3], logit_bias={9: -INF, 3: -INF}), dict(logit_bias=every)):
+        with pytest.raises(ValueError, match="no token is left"):
+            eng.sample(row, temperature, **kw)
+    assert eng.sample(row, temperature, allowed=[9, 3], logit_bias={9: -INF}) == 3
+    low = np.full(256, -INF, np.float32)
+    low[5] = 1.0
+    with pytest.raises(ValueError, match="no token is left"):   # (the model's own logits leave none of it)
+        eng.sample(low, temperature, allowed=[9, 200])
