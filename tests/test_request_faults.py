@@ -108,3 +108,25 @@ def test_a_request_that_no_token_is_left_to_ends_itself(tiny, temperature):  # n
     low[5] = 1.0
     with pytest.raises(ValueError, match="no token is left"):   # (the model's own logits leave none of it)
         eng.sample(low, temperature, allowed=[9, 200])
+
+
+def test_adapter_options_that_are_not_known_are_refused(tiny, tmp_path):  # noqa: F811
+    import request_ops as ro
+    from ninfer_amd import WeightError
+    folder, cfg, _ = tiny
+    eng = engine(folder)
+    factors = ro.random_factors(ro.attention_shapes(cfg, [0], "q"), 4, 1)
+    for i, options in enumerate((dict(alora_invocation_tokens=[5, 6]), dict(some_new_option=True), dict(some_new_option="x"), dict(some_new_option=0.5),
+                                 dict(target_parameters=["mlp.experts.down_proj"]), dict(arrow_config={"top_k": 2}), dict(use_rslora="false"))):
+        with pytest.raises(WeightError, match=f"{next(iter(options))} ="):
+            eng.load_adapter("bad", ro.write_adapter(tmp_path / f"bad{i}", factors, 4, 4, **options))
+    assert eng.adapters() == []
+    # what training libraries write beside the options that count, and options that are off
+    usual = dict(alora_invocation_tokens=None, alpha_pattern={}, arrow_config=None, auto_mapping=None, base_model_name_or_path="some/model", corda_config=None,
+                 ensure_weight_tying=False, eva_config=None, exclude_modules=["lm_head"], fan_in_fan_out=False, inference_mode=True, init_lora_weights=True,
+                 layer_replication=None, layers_pattern=None, layers_to_transform=None, loftq_config={}, lora_bias=False, lora_dropout=0.05,
+                 megatron_config=None, megatron_core="megatron.core", modules_to_save=None, peft_version="0.18.0", qalora_group_size=16, rank_pattern={},
+                 revision=None, runtime_config={"ephemeral_gpu_offload": False}, target_modules=["q_proj"], target_parameters=None, task_type="CAUSAL_LM",
+                 trainable_token_indices=None, use_qalora=False, use_rslora=False, some_new_option=None, another=False, a_third=[], a_fourth={})
+    eng.load_adapter("fine", ro.write_adapter(tmp_path / "fine", factors, 4, 4, **usual))
+    assert eng.adapters() == ["fine"]
