@@ -71,6 +71,7 @@ class AdapterSet:
         if problems:
             raise WeightError(f"adapter {name!r}: " + "; ".join(problems))
         g, r = self._names.index(None), weights.rank
+        self._wait()
         for s in self.spots:
             t, at, here = s.tables, 0, False
             t.a[g].zero_()
@@ -84,8 +85,7 @@ class AdapterSet:
                 at += columns
             t.ranks[g] = r if here else 0
         self._scale[g] = weights.scale
-        if self._scale.is_cuda:
-            torch.cuda.synchronize(self._scale.device)   # (steps on any stream find it)
+        self._wait()   # (steps on any stream find it)
         self._names[g], self._holds[g] = name, 0
         return g
 
@@ -94,9 +94,15 @@ class AdapterSet:
         g = self.number(name)
         if self._holds[g]:
             raise ValueError(f"adapter {name!r} is in use ({self._holds[g]} open requests or sessions)")
+        self._wait()
         for s in self.spots:
             s.tables.ranks[g] = 0
         self._names[g] = None
+
+    def _wait(self) -> None:
+        """Before a place's numbers change: a step that nobody has read back may still read them, on whatever stream."""
+        if self._scale.is_cuda:
+            torch.cuda.synchronize(self._scale.device)
 
     def hold(self, name: str) -> None:
         self._holds[self.number(name)] += 1

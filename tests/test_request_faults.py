@@ -130,3 +130,31 @@ def test_adapter_options_that_are_not_known_are_refused(tiny, tmp_path):  # noqa
                  trainable_token_indices=None, use_qalora=False, use_rslora=False, some_new_option=None, another=False, a_third=[], a_fourth={})
     eng.load_adapter("fine", ro.write_adapter(tmp_path / "fine", factors, 4, 4, **usual))
     assert eng.adapters() == ["fine"]
+
+
+def test_a_place_changes_only_after_the_steps_that_read_it(tiny, tmp_path, monkeypatch):  # noqa: F811
+    """Loading and removing wait for the device before they write, and loading after that too (tables that say they are on a GPU; the waits
+    are counted and see what has been written)."""
+    import torch
+
+    class OnGpu(torch.Tensor):
+        is_cuda = True
+
+    folder, cfg, _ = tiny
+    eng = engine(folder, max_adapters=1)
+    made = adapters_of(tmp_path, cfg)
+    held = eng.runner.adapters
+    held._scale = torch.Tensor._make_subclass(OnGpu, held._scale)
+    numbers = lambda: [t.clone() for s in held.spots for t in (s.tables.a, s.tables.b, s.tables.ranks)] + [held._scale.clone()]
+    same = lambda x, y: all(torch.equal(a, b) for a, b in zip(x, y))
+    waits = []
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda device=None: waits.append(numbers()))
+    for name in ("all", "o"):
+        before = numbers()
+        eng.load_adapter(name, made[name][0])
+        assert len(waits) == 2 and same(waits[0], before) and same(waits[1], numbers()) and not same(before, numbers())
+        waits.clear()
+        before = numbers()
+        eng.remove_adapter(name)
+        assert len(waits) == 1 and same(waits[0], before) and not same(before, numbers())
+        waits.clear()
