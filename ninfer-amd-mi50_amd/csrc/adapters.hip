@@ -14,9 +14,9 @@
 // the host no list of groups, so that a captured step serves whatever requests come.
 //
 // What bounds it: few rows, the latency of two launches that each wait for memory once (the factors
-// of the step's adapters are some MB: 64 rows of three slices of 2,048 numbers and eight adapters of ranks up to 64, 13 us in a
+// of the step's adapters are some MB: 64 rows of three slices of 2,048 numbers and eight adapters of ranks up to 64, 15 us in a
 // captured step; one row of rank 16, in one launch, 7); many rows, reading and writing x, base and out (2,055 rows of 3,584
-// numbers: 33 us, 1.9 TB/s of what cannot be spared: both launches wait for rows and factors in turn). h of bfloat16 rows enters the
+// numbers: 34 us, 1.8 TB/s of what cannot be spared: both launches wait for rows and factors in turn). h of bfloat16 rows enters the
 // second product as a sum of three bfloat16 numbers (the rounded value, what the rounding left, rounded, and what that left: 8 bits
 // each, 24 together), so that none of its bits is lost and `out` alone is rounded.
 //
@@ -209,7 +209,7 @@ __device__ __forceinline__ void wave_fence() {
 
 // Rows on their way to the matrix units pass through shared memory of the wave: there a lane needs 16 bytes of row `lane % 16`, and
 // such loads, whose neighbouring lanes read different rows, cost the cache four times what loads of whole lines do (2,055 rows of
-// 3,584 numbers, the first product: 42 us so, 18 through shared memory; the second 26 and 17). 16 rows of 128 bytes, eight pieces each: piece c of row r lies at 8 r + (c ^ r / 2),
+// 3,584 numbers, the first product: 42 us so, 18 through shared memory; the second, with h in two numbers, 26 and 17). 16 rows of 128 bytes, eight pieces each: piece c of row r lies at 8 r + (c ^ r / 2),
 // so that sixteen rows' pieces of one number lie in different banks. A lane loads (and puts) piece lane % 8 of rows lane / 8 and
 // lane / 8 + 8.
 __device__ __forceinline__ int place8(int row, int piece) { return row * 8 + (piece ^ (row >> 1)); }
@@ -558,8 +558,8 @@ __global__ __launch_bounds__(kExpandWaves * 64, RT == 1 ? 4 : 3) void adapter_ex
 // Up to 16 rows and ranks up to kFewRank in one launch: a block makes the h that its columns (512 of a slice) need itself, into its
 // own memory, in the order of the other kernels' sums. The factor A is read by every block of its slice, out of L2; what this saves
 // is a launch and the wait for the first one's end. us in one and in two launches, rows of 2,048 numbers, adapters of their own: rank
-// 16, 2,048 columns, one row 6.8 and 8.4; 3 x 2,048, 8 rows 10.0 and 10.9. With larger ranks every block has too much to read: rank
-// 64, 3 x 2,048 columns, one row 10.4 and 9.1, 16 rows 14.1 and 11.5.
+// 16, 2,048 columns, one row 7.0 and 8.3; 3 x 2,048, 8 rows 10.2 and 10.9, 16 rows 13.3 and 14.2. With larger ranks every block has too
+// much to read (with h in two numbers: rank 64, 3 x 2,048 columns, one row 10.4 and 9.1, 16 rows 14.1 and 11.5).
 constexpr int kFewRows = 16, kFewRank = 16;
 
 template <typename T, Rows ROWS, bool VEC, typename O = T>
@@ -600,13 +600,14 @@ __global__ __launch_bounds__(kWaves * 64, 2) void adapter_few_kernel(const Adapt
   }
 }
 
-// The grid of a kernel for which the tiles' first adapters are `total` blocks' work.
+// The grid of a kernel for which the tiles' first adapters are `total` blocks' work. Tiles of 32 rows: a block a CU more looks for
+// further ones (fewer than that only where fewer can be there).
 template <int RT>
 static dim3 grid_of(const AdapterArgs& a, int total, int* more) {
   static_assert(RT == 1 || RT == 2, "find_further looks at tiles of 32 rows");
   const int most = std::min(std::min(16 * RT, a.T), a.L), cus = device_cu_count();   // adapters that a tile may have
   if (RT == 1) return dim3(total, std::max(1, std::min(most, 4 * cus / total)));
-  if (most > 1) *more = (int)std::min<long long>((most - 1ll) * total, std::max(cus - total, cus));
+  if (most > 1) *more = (int)std::min<long long>((most - 1ll) * total, cus);
   return dim3((total + kXcds - 1) / kXcds * kXcds + *more);
 }
 
@@ -659,18 +660,20 @@ static void few(const AdapterArgs& a, const Forms<T, O>& f, hipStream_t stream) 
   else adapter_few_kernel<T, kWhole, true, O><<<grid, kWaves * 64, 0, stream>>>(a, f.sets, f.out);
 }
 
-// Blocks of 32 rows and 64 columns of the first product from which these are the faster ones: blocks of 16 by 16 are many more. us of both
-// products so and in blocks of 16 by 16: bfloat16, 3 x 64 columns of 2,048, 384 rows 15.7 and 13.3, 512 (48 blocks) 15.8 and 14.0, with
-// eight single rows before them 23.4 and 26.9, 1,024 rows 19.2 and 20.4, 26.5 and 39.4; 3 x 16 columns, 1,024 rows (32) 17.4 and 14.7; 32-bit,
-// 3 x 64 columns, 1,024 rows (96) 48 and 37, 2,048 (192) 64 and 64, with eight single rows 74 and 91. Rows that each have an adapter of
-// their own never: 512 of eight adapters in turn 97 and 60.
+// Blocks of 32 rows and 64 columns of the first product from which these are taken; blocks of 16 by 16 are many more. A portion alone is
+// faster in them from some 64 on (in 32 bits 192), but single rows before it, which steps of an engine have, gain more from them below
+// that than the portion alone loses. us of both products so and in blocks of 16 by 16, portions alone and with eight single rows of
+// other adapters before them: bfloat16, 3 x 64 columns of 2,048, 384 rows 16.0 and 13.6, 23.4 and 25.3; 512 (48 blocks) 16.3 and 14.6, 23.9
+// and 29.1; 768 19.1 and 20.3, 26.1 and 42.3; 2,048 27.5 and 34.7, 35.5 and 51.8; 3 x 16 columns, 1,024 rows (32) 18.2 and 14.9, 23.7 and
+// 22.3, 2,048 (64) 24.3 and 23.6, 30.7 and 35.5; 32-bit, 3 x 64 columns, 1,024 rows (96) 48 and 37, 58 and 79, 2,048 (192) 64.9 and 64.5, 73
+// and 95. Rows that each have an adapter of their own never: 512 of eight adapters in turn 100 and 63.
 template <typename T> constexpr int kManyBlocks = sizeof(T) == 2 ? 48 : 192;
 
 // The second product in tiles of 32 rows once these make three blocks for four CUs: as fast as in tiles of 16 where every tile has one
 // adapter, and faster by what a tile of single rows takes that has several, whose further ones are blocks of their own here and
 // one pass after the other there. us in tiles of 32 and of 16, bfloat16, 3 x 2,048 columns, rank 16, eight single rows before 256 rows of one
-// request 15.2 and 18.9, 512 16.2 and 27.8, 1,024 21 and 33, without the single rows 9.7 and 9.9, 11.0 and 11.1, 14.7 and 17.0; 32-bit,
-// rank 64, 256 rows 33 and 40, without 18.9 and 17.1.
+// request 16.0 and 21.3, 512 17.4 and 31.8, 1,024 23 and 37, without the single rows 9.9 and 10.0, 11.3 and 11.2, 14.8 and 16.9; 32-bit,
+// rank 64, 256 rows 33 and 44, without 18.9 and 17.1.
 static bool tiles_of_32(const AdapterArgs& a, int sets) {
   return !a.single && (a.T + 31ll) / 32 * ((sets + kExpandWaves - 1) / kExpandWaves) * 4 >= 3ll * device_cu_count();
 }

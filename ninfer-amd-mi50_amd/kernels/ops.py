@@ -2303,8 +2303,8 @@ class HipOps:
         h, of_row = self._adapter_scratch(x, slices, r)
         lib, stream, code, ph = self.lib, self._stream_of(dev), _DT[dt], 0 if h is None else h.data_ptr()
         # (Single rows of many adapters beside other rows: two calls, since a tile of theirs has an adapter a row. us so and in one call, 64
-        # adapters of rank 16 beside q, k and v of 2,048 columns: 32 of them and 512 rows 27 and 39, 2,048 rows 39 and 49; 8 of them 21 and
-        # 16, 34 and 30.)
+        # adapters of rank 16 beside q, k and v of 2,048 columns: 32 of them and 512 rows 28 and 39, 2,048 rows 40 and 50; 8 of them 22 and
+        # 16, 35 and 31.)
         apart = min(single_rows, count) >= 16 and t - single_rows >= 128
         for lo, hi in ((0, single_rows), (single_rows, t)) if apart else ((0, t),):
             args = _ADAPTER_ARGS.pack(px + lo * ldx * size, *tables, p_rows + 4 * lo, pb + lo * ldb * size, po + lo * ldo * size,
