@@ -713,6 +713,7 @@ static int check_adapters(const AdapterArgs* args, bool alone) {
   NINFER_REQUIRE(args, "adapter_add: no arguments");
   const AdapterArgs& a = *args;
   NINFER_REQUIRE(a.T > 0 && a.K > 0 && a.R > 0 && a.L > 0, "adapter_add: T=%d K=%d R=%d L=%d must be positive", a.T, a.K, a.R, a.L);
+  NINFER_REQUIRE(a.K <= 0x7fffffff - 128, "adapter_add: rows of %d numbers are too long", a.K);   // (steps are counted past the row's end)
   NINFER_REQUIRE(a.S >= 1 && a.S <= 4 && a.first[0] == 0 && a.first[a.S] == a.N, "adapter_add: %d slices of %d columns", a.S, a.N);
   for (int s = 0; s < a.S; ++s)
     NINFER_REQUIRE(a.first[s] < a.first[s + 1], "adapter_add: slice %d has no columns", s);

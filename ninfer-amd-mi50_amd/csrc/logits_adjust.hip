@@ -285,6 +285,7 @@ extern "C" int ninfer_adjust_logits(const AdjustArgs* args, hipStream_t stream) 
   NINFER_REQUIRE(args, "adjust_logits: no arguments");
   AdjustArgs a = *args;
   NINFER_REQUIRE(a.R > 0 && a.V > 0 && a.logits && a.out, "adjust_logits: R=%d V=%d must be positive, rows not null", a.R, a.V);
+  NINFER_REQUIRE(a.V <= 0x7fffffff - kAdjustPart, "adjust_logits: rows of %d tokens are too long", a.V);   // (parts are counted past the row's end)
   NINFER_REQUIRE(a.ld >= a.V && a.ldo >= a.V, "adjust_logits: row stride %lld or %lld < vocabulary %d", a.ld, a.ldo, a.V);
   NINFER_REQUIRE(a.logits != a.out || a.ld == a.ldo, "adjust_logits: in place with two row strides");
   NINFER_REQUIRE(a.n_hist >= 0 && a.n_bias >= 0 && a.n_masks >= 0, "adjust_logits: a size is negative");

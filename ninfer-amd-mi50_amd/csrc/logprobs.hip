@@ -29,6 +29,7 @@ constexpr int kLpPart = kLpThreads * kLpQuads * 4;
 constexpr int kLpTop = 64;          // most tokens that are listed: the groups the bound is taken from
 constexpr int kLpJoinThreads = 1024;
 constexpr int kLpSegments = 256;    // most threads of the first launch whose logits are looked at again
+constexpr int kLpMostTokens = 0x7fffffff - kLpPart;   // (a turn's and a part's tokens are counted past the row's end)
 constexpr int kLpFound = 1024;      // ... and most of these logits that reach the bound
 
 struct LogprobArgs {
@@ -311,6 +312,7 @@ extern "C" int ninfer_token_logprobs(const LogprobArgs* args, void* scratch, hip
   NINFER_REQUIRE(args && scratch && (uintptr_t)scratch % 16 == 0, "token_logprobs: no arguments, or scratch not aligned");
   LogprobArgs a = *args;
   NINFER_REQUIRE(a.R > 0 && a.V > 0 && a.logits, "token_logprobs: R=%d V=%d must be positive, rows not null", a.R, a.V);
+  NINFER_REQUIRE(a.V <= kLpMostTokens, "token_logprobs: rows of %d tokens are too long", a.V);
   NINFER_REQUIRE(a.ld >= a.V, "token_logprobs: row stride %lld < vocabulary %d", a.ld, a.V);
   NINFER_REQUIRE(a.top >= 0 && a.top <= kLpTop && a.top <= a.V, "token_logprobs: top %d is outside [0, min(%d, %d)]", a.top, kLpTop, a.V);
   NINFER_REQUIRE(!a.tokens || (a.logprob && a.before), "token_logprobs: tokens without a place for their numbers");

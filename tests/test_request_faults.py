@@ -1,9 +1,10 @@
 """Requests whose options, or whose steps, fail: what they are told, and what is left behind them (on the CPU, with plain twins of the kernels)."""
+import ctypes
 import math
 
 import pytest
 
-from test_requests import adapters_of, engine, greedy, tiny  # noqa: F401
+from test_requests import adapters_of, engine, greedy, lib, refuses, tiny  # noqa: F401
 
 INF, NAN = math.inf, math.nan
 
@@ -158,3 +159,15 @@ def test_a_place_changes_only_after_the_steps_that_read_it(tiny, tmp_path, monke
         eng.remove_adapter(name)
         assert len(waits) == 1 and same(waits[0], before) and not same(before, numbers())
         waits.clear()
+
+
+def test_rows_too_long_to_count_past_their_end_are_refused(lib):  # noqa: F811
+    """The last turn over a row, and its last part, are counted past the row's end in 32 bits."""
+    from ninfer_amd.kernels.ops import _ADAPTER_ARGS, _ADJUST_ARGS, _LOGPROB_ARGS
+    p, most = 1 << 20, 2 ** 31 - 1
+    for v in (most, most - 4095):
+        refuses(lib, lambda: lib.ninfer_token_logprobs(_LOGPROB_ARGS.pack(p, p, p, p, p, p, 0, 0, 0, most, 1, v, 1, 0), ctypes.c_void_p(p), None), "too long")
+        refuses(lib, lambda: lib.ninfer_adjust_logits(_ADJUST_ARGS.pack(p, p, *[0] * 12, most, most, 1, v, 0, 0, 0, 0), None), "too long")
+    for k in (most, most - 127):
+        refuses(lib, lambda: lib.ninfer_adapter_add(_ADAPTER_ARGS.pack(p, p, p, p, p, p, p, p, p, most, 64, 64, 1, k, 8, 1, 1, 64, 0, 64, 64, 64, 64, 1, 0), None),
+                "too long")
