@@ -167,7 +167,10 @@ def allowed_words(allowed, vocab: int) -> Optional[np.ndarray]:
         if vocab % 32:
             words[-1] &= np.uint32((1 << vocab % 32) - 1)
     else:
-        ids = np.asarray(list(allowed), dtype=np.int64)
+        ids = np.asarray(list(allowed))
+        if ids.dtype == np.bool_:   # (as ids they would be tokens 0 and 1)
+            raise ValueError("allowed tokens are ids or the words of a mask, not truth values")
+        ids = ids.astype(np.int64)
         if ids.size and not (0 <= ids.min() and ids.max() < vocab):
             raise ValueError(f"an allowed token is outside [0, {vocab})")
         words = np.zeros(n, np.uint32)

@@ -171,3 +171,19 @@ def test_rows_too_long_to_count_past_their_end_are_refused(lib):  # noqa: F811
     for k in (most, most - 127):
         refuses(lib, lambda: lib.ninfer_adapter_add(_ADAPTER_ARGS.pack(p, p, p, p, p, p, p, p, p, most, 64, 64, 1, k, 8, 1, 1, 64, 0, 64, 64, 64, 64, 1, 0), None),
                 "too long")
+
+
+def test_truth_values_are_no_allowed_tokens(tiny):  # noqa: F811
+    import numpy as np
+    import torch
+    from ninfer_amd.sampling.sampler import allowed_words
+    for mask in ([True, False] * 20, np.ones(40, bool), torch.ones(40, dtype=torch.bool)):
+        with pytest.raises(ValueError, match="truth values"):
+            allowed_words(mask, 40)
+    for ids in ([3, 5], (3, 5), {3, 5}, np.array([3, 5], np.int32), torch.tensor([5, 3]), iter([5, 3]), range(3, 6, 2)):
+        assert allowed_words(ids, 40).tolist() == [1 << 3 | 1 << 5, 0]
+    with pytest.raises(ValueError, match="no token"):
+        allowed_words([], 40)
+    eng = engine(tiny[0])
+    with pytest.raises(RuntimeError, match="truth values"):
+        eng.generate([[1, 2]], greedy(2), [], None, [lambda out: np.arange(256) > 9])
