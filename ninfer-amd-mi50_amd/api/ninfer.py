@@ -265,7 +265,7 @@ class Ninfer:
                 sched.add(r)
             sched.run()
         except BaseException as e:   # (the scheduler ends with this call: nothing may stay held by its requests)
-            sched.abort(str(e))
+            sched.abort(str(e) or type(e).__name__)
             raise
         for r in reqs:
             if r.status == "failed":
